@@ -132,6 +132,7 @@ SIGNATURES = {
     "cdae_causal_mask": [P, P, P, I, I, I, I, P],
     "cdae_adamw_ema": [P, P, P, P, P, L, D, D, D, D, D, I, D, D, P],
     "cdae_adamw_ema_multi": [P, P, P, P, P, P, I, L, D, D, D, D, D, I, D, P],
+    "cdae_adamw_ema_factor": [P, P, P, P, P, P, I, L, D, D, D, D, D, I, P, P],
     "cdae_sqsum": [P, L, P, P],
     "cdae_p_mean_variance": [P, P, P, P, I, I, I, I, P, P, P, P, P, P, I, L, P],
     "cdae_vb_terms": [P, P, P, P, P, I, I, I, I, P, P, I, L, P],
@@ -163,6 +164,15 @@ SIGNATURES = {
     "cdae_upsample2_16": [P, P, I, I, I, I, P],
     "cdae_sumpool2_16": [P, P, I, I, I, I, P],
     "cdae_wprep_all_m16": [P, P, I, I, L, P, P, P, P, P, P, P, P, P, P],
+    "cdae_lin16_workspace_bytes": [I, I, I, I],
+    "cdae_lin16_fwd": [P, L, P, L, P, P, L, P, L, P, L, I, I, I, I, I, P, SZ, P],
+    "cdae_lin16_bwd": [P, L, P, L, P, L, P, L, P, L, P, L, P, I, I, I, I, I, P, SZ, P],
+    "cdae_resnorm_workspace_bytes": [I, I, I],
+    "cdae_resnorm_fwd": [P, P],
+    "cdae_resnorm_bwd": [P, P],
+    "cdae_grad_workspace_bytes": [],
+    "cdae_grad_norm": [P, P, P, I, D, D, P, P, SZ, P],
+    "cdae_grad_clip": [P, P, P, P, P, I, D, D, P, P, SZ, P],
     "cdae_tune_set": [I, I],
     "cdae_tune_get": [I],
     "cdae_prof_enable": [I],
@@ -170,7 +180,8 @@ SIGNATURES = {
     "cdae_calib_mfma": [P, SZ, I, P, P, P],
     "cdae_calib_copy": [P, P, SZ, I, P, P],
 }
-_RESTYPES = {"cdae_last_error": ctypes.c_char_p, "cdae_gn_workspace_floats": SZ, "cdae_bn_workspace_floats": SZ, "cdae_workspace_bytes": SZ}
+_RESTYPES = {"cdae_last_error": ctypes.c_char_p, "cdae_gn_workspace_floats": SZ, "cdae_bn_workspace_floats": SZ, "cdae_workspace_bytes": SZ, "cdae_lin16_workspace_bytes": SZ,
+             "cdae_resnorm_workspace_bytes": SZ, "cdae_grad_workspace_bytes": SZ}
 
 TAB_ROWS = 12
 PROF_FAMILIES = ("igemm", "groupnorm", "softmax", "elementwise", "optimizer", "convwin", "convwin_dgrad", "convwin_up")
@@ -189,6 +200,15 @@ class WgItem(ctypes.Structure):
     """cdae_wg_item (include/cdae.h): one weight gradient of a group launch"""
     _fields_ = [("a_hi", P), ("a_lo", P), ("dy_hi", P), ("dy_lo", P), ("dw", P), ("dbias", P),
                 ("N", I), ("H", I), ("W", I), ("Cin", I), ("Cout", I), ("accumulate", I)]
+
+
+class ResNorm(ctypes.Structure):
+    """cdae_resnorm (include/cdae.h): the arguments of the norms around a block"""
+    _fields_ = ([(n, I) for n in ("B", "T", "C", "dt", "layer", "post", "pre", "vec32", "w32", "shared_gate", "shared_scale", "shared_shift")]
+                + [("alpha", F), ("eps", F)] + [(n, P) for n in ("x", "f", "gate", "scale", "shift", "w1", "b1", "w2", "b2")]
+                + [(n, L) for n in ("ld_x", "ld_f", "ld_gate", "ld_scale", "ld_shift")] + [(n, P) for n in ("r", "u", "dr", "du")]
+                + [("ld_dr", L), ("ld_du", L)] + [(n, P) for n in ("dx", "df", "dgate", "dscale", "dshift", "dw1", "db1", "dw2", "db2")]
+                + [("ws", P), ("ws_bytes", SZ)])
 
 
 def _load():

@@ -1,0 +1,59 @@
+// Element access shared by the transformer-block kernels (lin16.hip, resnorm.hip, gradclip.hip): bf16 / f16 / fp32 values as fp32 in registers.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+enum { DT_BF16 = 0, DT_F16 = 1, DT_F32 = 2 };
+
+struct Bf16 { unsigned short u; };
+struct F16 { _Float16 h; };
+
+__device__ __forceinline__ float ld1(Bf16 v) { return __builtin_bit_cast(float, (unsigned)v.u << 16); }
+__device__ __forceinline__ float ld1(F16 v) { return (float)v.h; }
+__device__ __forceinline__ float ld1(float v) { return v; }
+__device__ __forceinline__ void st1(Bf16& d, float v) { d.u = __builtin_bit_cast(unsigned short, (__bf16)v); }       // round to nearest even
+__device__ __forceinline__ void st1(F16& d, float v) { d.h = (_Float16)v; }
+__device__ __forceinline__ void st1(float& d, float v) { d = v; }
+
+// V consecutive values at ANY element alignment: the vector type carries the element's alignment, so rows of an odd length are read with the
+// same wide instructions as aligned ones
+template <class T, int V>
+struct __attribute__((packed, aligned(sizeof(T)))) Pack { T v[V]; };
+
+template <class T, int V>
+__device__ __forceinline__ void ldv(const T* __restrict__ p, float (&o)[V]) {
+    const Pack<T, V> t = *reinterpret_cast<const Pack<T, V>*>(p);
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = ld1(t.v[i]);
+}
+template <class T, int V>
+__device__ __forceinline__ void stv(T* __restrict__ p, const float (&o)[V]) {
+    Pack<T, V> t;
+#pragma unroll
+    for (int i = 0; i < V; ++i) st1(t.v[i], o[i]);
+    *reinterpret_cast<Pack<T, V>*>(p) = t;
+}
+// the same with only the first n (0..V) values present; the others read as zero and are not written
+template <class T, int V>
+__device__ __forceinline__ void ldv_n(const T* __restrict__ p, int n, float (&o)[V]) {
+    if (n >= V) { ldv<T, V>(p, o); return; }
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = i < n ? ld1(p[i]) : 0.f;
+}
+template <class T, int V>
+__device__ __forceinline__ void stv_n(T* __restrict__ p, int n, const float (&o)[V]) {
+    if (n >= V) { stv<T, V>(p, o); return; }
+#pragma unroll
+    for (int i = 0; i < V; ++i) if (i < n) st1(p[i], o[i]);
+}
+// a vector kept either in the rows' type T or in fp32 (a uniform choice)
+template <class T, int V>
+__device__ __forceinline__ void ldv_n2(const void* __restrict__ p, long off, int is32, int n, float (&o)[V]) {
+    if (is32) ldv_n<float, V>(reinterpret_cast<const float*>(p) + off, n, o);
+    else ldv_n<T, V>(reinterpret_cast<const T*>(p) + off, n, o);
+}
+template <class T>
+__device__ __forceinline__ void st2(void* p, long off, int is32, float v) {
+    if (is32) reinterpret_cast<float*>(p)[off] = v;
+    else st1(reinterpret_cast<T*>(p)[off], v);
+}

@@ -6,7 +6,7 @@ cd "$(dirname "$0")"
 OUT=../libcdae.so
 HIPCC=${HIPCC:-/opt/rocm/bin/hipcc}
 FLAGS="${EXTRA_HIPCC_FLAGS:-} --offload-arch=gfx950 -O3 -fPIC -std=c++17 -Wall -Wno-unused-function -Wno-inline-asm -Wno-unused-command-line-argument -Xclang -target-feature -Xclang -packed-fp32-ops -I../../include"
-UNITS="igemm planes api norm elementwise prof attention attn16 rows16 wg16 wgrad stem convwin skipgn head"
+UNITS="igemm planes api norm elementwise prof attention attn16 rows16 wg16 wgrad stem convwin skipgn head lin16 resnorm gradclip"
 mkdir -p build
 # (the flag record is written only after every compile step has succeeded: a failed build after a flag change must not leave
 #  objects of the old flag set looking current)
@@ -14,7 +14,7 @@ if [ "$(cat build/.flags 2>/dev/null || true)" != "$FLAGS" ]; then FORCE=1; rm -
 pids=()
 for u in $UNITS; do
     obj=build/$u.o
-    if [ "${FORCE:-0}" = 1 ] || [ ! -f $obj ] || [ $u.hip -nt $obj ] || [ cdae_internal.h -nt $obj ] || [ gemm_common.h -nt $obj ] || [ ../../include/cdae.h -nt $obj ]; then
+    if [ "${FORCE:-0}" = 1 ] || [ ! -f $obj ] || [ $u.hip -nt $obj ] || [ cdae_internal.h -nt $obj ] || [ gemm_common.h -nt $obj ] || [ block_common.h -nt $obj ] || [ ../../include/cdae.h -nt $obj ]; then
         extra=""
         [ $u = elementwise ] && extra="-ffp-contract=off"       # sampler updates round like the reference's separate ATen ops
         $HIPCC $FLAGS $extra -c $u.hip -o $obj & pids+=($!)

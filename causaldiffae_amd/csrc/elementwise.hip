@@ -620,7 +620,8 @@ __global__ void adamw_ema_kernel(float* __restrict__ p, const float* __restrict_
 struct EmaSet { float* buf[4]; float rate[4]; int n; };
 __global__ void adamw_ema_multi_kernel(float* __restrict__ p, const float* __restrict__ g, float* __restrict__ m, float* __restrict__ v,
                                        EmaSet es, long n, float lr, float b1, float b2, float eps, float wd,
-                                       float bc1, float sqrt_bc2, float grad_scale) {
+                                       float bc1, float sqrt_bc2, float grad_scale, const float* __restrict__ factor) {
+    if (factor) grad_scale = *factor;            // (clipping: the factor was computed on the device)
     GRID_STRIDE(i, n) {
         float gi = g[i] * grad_scale;
         float pi = p[i] * (1.f - lr * wd);
@@ -1048,8 +1049,8 @@ int cdae_adamw_ema(float* p, const float* g, float* m, float* v, float* ema, lon
     if (hipGetLastError() != hipSuccess) return cdae_fail("adamw_ema launch failed");
     return 0;
 }
-int cdae_adamw_ema_multi(float* p, const float* g, float* m, float* v, float* const* emas, const double* ema_rates, int n_ema, long n, double lr,
-                         double beta1, double beta2, double eps, double weight_decay, int step, double grad_scale, void* stream) {
+static int adamw_ema_launch(float* p, const float* g, float* m, float* v, float* const* emas, const double* ema_rates, int n_ema, long n, double lr,
+                            double beta1, double beta2, double eps, double weight_decay, int step, double grad_scale, const float* factor, void* stream) {
     if (n_ema < 0 || n_ema > 4 || (n_ema && (!emas || !ema_rates))) return cdae_fail("adamw_ema_multi: 0..4 EMA buffers (host arrays of pointers and rates)");
     EmaSet es{};
     es.n = n_ema;
@@ -1058,10 +1059,19 @@ int cdae_adamw_ema_multi(float* p, const float* g, float* m, float* v, float* co
     const float sqrt_bc2 = (float)sqrt(1.0 - pow(beta2, (double)step));
     cdae_prof_begin(PROF_OPT, (double)n * (24.0 + 8.0 * n_ema), ST);
     hipLaunchKernelGGL(adamw_ema_multi_kernel, dim3(grid_for(n, 8192)), dim3(256), 0, ST, p, g, m, v, es, n, (float)lr, (float)beta1, (float)beta2, (float)eps,
-                       (float)weight_decay, bc1, sqrt_bc2, (float)grad_scale);
+                       (float)weight_decay, bc1, sqrt_bc2, (float)grad_scale, factor);
     cdae_prof_end(PROF_OPT, ST);
     if (hipGetLastError() != hipSuccess) return cdae_fail("adamw_ema_multi launch failed");
     return 0;
+}
+int cdae_adamw_ema_multi(float* p, const float* g, float* m, float* v, float* const* emas, const double* ema_rates, int n_ema, long n, double lr,
+                         double beta1, double beta2, double eps, double weight_decay, int step, double grad_scale, void* stream) {
+    return adamw_ema_launch(p, g, m, v, emas, ema_rates, n_ema, n, lr, beta1, beta2, eps, weight_decay, step, grad_scale, nullptr, stream);
+}
+int cdae_adamw_ema_factor(float* p, const float* g, float* m, float* v, float* const* emas, const double* ema_rates, int n_ema, long n, double lr,
+                          double beta1, double beta2, double eps, double weight_decay, int step, const float* factor, void* stream) {
+    if (!factor) return cdae_fail("adamw_ema_factor: a factor in device memory required");
+    return adamw_ema_launch(p, g, m, v, emas, ema_rates, n_ema, n, lr, beta1, beta2, eps, weight_decay, step, 1.0, factor, stream);
 }
 int cdae_sqsum(const float* x, long n, double* out, void* stream) {
     if (hipMemsetAsync(out, 0, sizeof(double), ST) != hipSuccess) return cdae_fail("memset failed");

@@ -1,0 +1,278 @@
+// gradclip.hip — the global norm of many gradients, and clipping by it (gfx950):
+//
+//     n = |scale| * sqrt(sum over all tensors of g^2),      out = g * scale * min(1, max_norm / (n + 1e-6))
+//
+// An HBM stream: the norm reads every gradient once, the clipping reads it again and writes it.  Squares are formed and added in fp64: fp32
+// squares leave their range at |g| > 1.8e19 and |g| < 1e-23, and 64-bit adds make the order of summation irrelevant at fp32 accuracy; the
+// fp64 pipe has room for it (one fma per 2..4 bytes read).  The order is fixed all the same: each block leaves ONE partial sum in a slot of
+// its own, every block of the second launch adds the slots in the same order, so the result is the same in every run.
+// Tensors come as kernel arguments, so the calls allocate nothing, copy nothing to the device and can be captured; back-to-back tensors (the
+// views of a flat buffer) are joined on the host and cost one table entry together.
+#include <hip/hip_runtime.h>
+#include <algorithm>
+#include <math.h>
+#include <vector>
+
+#include "cdae.h"
+#include "block_common.h"
+#include "cdae_internal.h"
+
+namespace {
+
+constexpr int GC_MAX = 144;                 // table entries of one launch: 144 * 25 + 4 bytes of arguments, below the 4 KB a launch may carry
+constexpr int GC_CHUNK = 16384;             // values a block takes at a time
+constexpr int GC_BLOCKS = 1024;             // blocks over all launches of a call, about four per CU
+constexpr int GC_SLOTS = 8192;              // partial sums the workspace holds: GC_BLOCKS + one more launch's minimum per table
+
+struct GcTab {
+    const void* in[GC_MAX];
+    void* out[GC_MAX];
+    long n[GC_MAX];
+    unsigned char types[GC_MAX];            // type of in | type of out << 4
+    int count;
+};
+static_assert(sizeof(GcTab) <= 3800, "kernel arguments");
+
+// (double sum) of one chunk
+template <class T>
+__device__ double sq_chunk(const T* __restrict__ p, long n) {
+    constexpr int V = 16 / sizeof(T);
+    double s0 = 0.0, s1 = 0.0;
+    long i = (long)threadIdx.x * V;
+    for (; i + V <= n; i += 256 * V) {
+        float v[V];
+        ldv<T, V>(p + i, v);
+#pragma unroll
+        for (int e = 0; e < V; e += 2) { s0 = fma((double)v[e], (double)v[e], s0); s1 = fma((double)v[e + 1], (double)v[e + 1], s1); }
+    }
+    for (long k = i; k < n && k < i + V; ++k) { const double v = ld1(p[k]); s0 = fma(v, v, s0); }
+    return s0 + s1;
+}
+
+__device__ double block_sum(double s) {
+    __shared__ double part[4];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+    __syncthreads();
+    s = (part[0] + part[1]) + (part[2] + part[3]);
+    __syncthreads();
+    return s;
+}
+
+// chunk c of the table: its entry and first value
+__device__ __forceinline__ bool find_chunk(const GcTab& t, long c, int& e, long& at) {
+    long first = 0;
+    for (e = 0; e < t.count; ++e) {
+        const long k = (t.n[e] + GC_CHUNK - 1) / GC_CHUNK;
+        if (c < first + k) { at = (c - first) * GC_CHUNK; return true; }
+        first += k;
+    }
+    return false;
+}
+
+__global__ __launch_bounds__(256) void gc_norm_kernel(const GcTab t, long chunks, double* __restrict__ slots) {
+    double s = 0.0;
+    for (long c = blockIdx.x; c < chunks; c += gridDim.x) {
+        int e; long at;
+        if (!find_chunk(t, c, e, at)) break;
+        const long n = t.n[e] - at < GC_CHUNK ? t.n[e] - at : GC_CHUNK;
+        const int ty = t.types[e] & 15;
+        if (ty == DT_F32) s += sq_chunk(reinterpret_cast<const float*>(t.in[e]) + at, n);
+        else if (ty == DT_BF16) s += sq_chunk(reinterpret_cast<const Bf16*>(t.in[e]) + at, n);
+        else s += sq_chunk(reinterpret_cast<const F16*>(t.in[e]) + at, n);
+    }
+    s = block_sum(s);
+    if (threadIdx.x == 0) slots[blockIdx.x] = s;
+}
+
+// every block adds all slots in the same order: norm and factor are the same bits everywhere
+__device__ double total(const double* __restrict__ slots, int nslots) {
+    double s = 0.0;
+    for (int i = threadIdx.x; i < nslots; i += 256) s += slots[i];
+    return block_sum(s);
+}
+__device__ __forceinline__ float clip_factor(double sum, double scale, double max_norm, float* norm) {
+    const double n = sqrt(sum) * fabs(scale);
+    *norm = (float)n;
+    const double c = max_norm / (n + 1e-6);
+    return (float)(scale * (c >= 1.0 ? 1.0 : c));           // (a norm that is not a number stays one in the factor)
+}
+
+__global__ __launch_bounds__(256) void gc_finish_kernel(const double* __restrict__ slots, int nslots, double scale, double max_norm, float* __restrict__ norm) {
+    const double s = total(slots, nslots);
+    if (threadIdx.x == 0) { float n; const float f = clip_factor(s, scale, max_norm, &n); norm[0] = n; norm[1] = f; }
+}
+
+template <class T, class O>
+__device__ void mul_chunk(const T* p, O* o, long n, float f) {
+    constexpr int V = 16 / sizeof(T);
+    long i = (long)threadIdx.x * V;
+    for (; i + V <= n; i += 256 * V) {
+        float v[V];
+        ldv<T, V>(p + i, v);
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] *= f;
+        stv<O, V>(o + i, v);
+    }
+    for (long k = i; k < n && k < i + V; ++k) st1(o[k], ld1(p[k]) * f);
+}
+template <class T>
+__device__ void mul_chunk_to(const T* p, void* o, int ty, long at, long n, float f) {
+    if (ty == DT_F32) mul_chunk(p + at, reinterpret_cast<float*>(o) + at, n, f);
+    else if (ty == DT_BF16) mul_chunk(p + at, reinterpret_cast<Bf16*>(o) + at, n, f);
+    else mul_chunk(p + at, reinterpret_cast<F16*>(o) + at, n, f);
+}
+
+__global__ __launch_bounds__(256) void gc_scale_kernel(const GcTab t, long chunks, const double* __restrict__ slots, int nslots, double scale, double max_norm,
+                                                       float* __restrict__ norm) {
+    float n;
+    const float f = clip_factor(total(slots, nslots), scale, max_norm, &n);
+    if (blockIdx.x == 0 && threadIdx.x == 0) { norm[0] = n; norm[1] = f; }
+    for (long c = blockIdx.x; c < chunks; c += gridDim.x) {
+        int e; long at;
+        if (!find_chunk(t, c, e, at)) break;
+        const int ti = t.types[e] & 15, to = t.types[e] >> 4;
+        if (f == 1.f && t.in[e] == t.out[e] && ti == to) continue;      // in place and nothing to clip: the values stay
+        const long left = t.n[e] - at < GC_CHUNK ? t.n[e] - at : GC_CHUNK;
+        if (ti == DT_F32) mul_chunk_to(reinterpret_cast<const float*>(t.in[e]), t.out[e], to, at, left, f);
+        else if (ti == DT_BF16) mul_chunk_to(reinterpret_cast<const Bf16*>(t.in[e]), t.out[e], to, at, left, f);
+        else mul_chunk_to(reinterpret_cast<const F16*>(t.in[e]), t.out[e], to, at, left, f);
+    }
+}
+
+int bytes_of(int ty) { return ty == DT_F32 ? 4 : 2; }
+
+// The next table of a list: joins entries that lie back to back (in and out, same types), skips empty ones.  -> entries used from `at`
+int fill(GcTab& t, const void* const* in, const long* n, const int* types, void* const* out, const int* out_types, int count, int at, long& chunks) {
+    t.count = 0;
+    chunks = 0;
+    int i = at;
+    for (; i < count; ++i) {
+        if (n[i] == 0) continue;
+        const unsigned char ty = (unsigned char)(types[i] | (out ? out_types[i] << 4 : 0));
+        if (t.count) {
+            const int k = t.count - 1;
+            if (t.types[k] == ty && (const char*)t.in[k] + t.n[k] * bytes_of(types[i]) == (const char*)in[i] &&
+                (!out || (char*)t.out[k] + t.n[k] * bytes_of(out_types[i]) == (char*)out[i])) {
+                t.n[k] += n[i];
+                continue;
+            }
+        }
+        if (t.count == GC_MAX) break;
+        t.in[t.count] = in[i];
+        t.out[t.count] = out ? out[i] : nullptr;
+        t.n[t.count] = n[i];
+        t.types[t.count] = ty;
+        ++t.count;
+    }
+    for (int k = 0; k < t.count; ++k) chunks += (t.n[k] + GC_CHUNK - 1) / GC_CHUNK;
+    return i;
+}
+
+int check_list(const char* what, const void* const* in, const long* n, const int* types, int count) {
+    if (count < 0 || (count && (!in || !n || !types))) return cdae_fail(what);
+    for (int i = 0; i < count; ++i)
+        if (n[i] < 0 || (n[i] && !in[i]) || types[i] < 0 || types[i] > 2) return cdae_fail(what);
+    return 0;
+}
+
+// Every output must be memory of its own, or exactly its input (in place): blocks write while others read, in no order.
+struct Span { const char* lo; const char* hi; int id; bool write; };
+int check_overlap(const void* const* in, const long* n, const int* types, void* const* out, const int* out_types, int count) {
+    try {
+        std::vector<Span> v;
+        v.reserve(2 * (size_t)count);
+        for (int i = 0; i < count; ++i) {
+            if (n[i] == 0) continue;
+            const char* a = (const char*)in[i];
+            const char* b = (const char*)out[i];
+            if (!(a == b && bytes_of(types[i]) == bytes_of(out_types[i]))) v.push_back({a, a + n[i] * bytes_of(types[i]), i, false});
+            v.push_back({b, b + n[i] * bytes_of(out_types[i]), i, true});
+        }
+        std::sort(v.begin(), v.end(), [](const Span& p, const Span& q) { return p.lo < q.lo; });
+        const char* wrote = nullptr;             // where the spans so far end: those written, those read
+        const char* read = nullptr;
+        for (const Span& s : v) {
+            if (s.lo < wrote || (s.write && s.lo < read)) return 1;
+            const char*& end = s.write ? wrote : read;
+            if (s.hi > end) end = s.hi;
+        }
+        return 0;
+    } catch (...) {
+        return 2;
+    }
+}
+
+// the norm launches: one partial sum a block, blocks shared out by each table's part of the values.  -> number of slots, or -1
+int launch_norm(const void* const* in, const long* n, const int* types, int count, double* slots, hipStream_t st) {
+    double all = 0.0;
+    for (int i = 0; i < count; ++i) all += (double)n[i];
+    int used = 0, at = 0;
+    while (at < count) {
+        GcTab t;
+        long chunks;
+        at = fill(t, in, n, types, nullptr, nullptr, count, at, chunks);
+        if (!t.count) break;
+        double mine = 0.0;
+        for (int k = 0; k < t.count; ++k) mine += (double)t.n[k];
+        long blocks = (long)(GC_BLOCKS * (mine / all)) + 1;
+        if (blocks > chunks) blocks = chunks;
+        if (used + blocks > GC_SLOTS) blocks = GC_SLOTS - used;
+        if (blocks < 1) { cdae_fail("grad_norm: too many tensors in one call"); return -1; }
+        hipLaunchKernelGGL(gc_norm_kernel, dim3((unsigned)blocks), dim3(256), 0, st, t, chunks, slots + used);
+        if (hipGetLastError() != hipSuccess) { cdae_fail("grad_norm launch failed"); return -1; }
+        used += (int)blocks;
+    }
+    return used;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t cdae_grad_workspace_bytes(void) { return sizeof(double) * GC_SLOTS; }
+
+int cdae_grad_norm(const void* const* in, const long* n, const int* types, int count, double scale, double max_norm, float* norm, void* ws, size_t ws_bytes,
+                   void* stream) {
+    if (check_list("grad_norm: a list of device tensors with sizes >= 0 and types 0 (bf16), 1 (fp16), 2 (fp32)", in, n, types, count)) return -1;
+    if (!norm || !ws || ws_bytes < cdae_grad_workspace_bytes()) return cdae_fail("grad_norm: norm[2] and a workspace of cdae_grad_workspace_bytes() required");
+    if (!(max_norm >= 0.0)) return cdae_fail("grad_norm: max_norm must be a number >= 0 (infinity: nothing is clipped)");
+    hipStream_t st = (hipStream_t)stream;
+    double* slots = (double*)ws;
+    const int used = launch_norm(in, n, types, count, slots, st);
+    if (used < 0) return -1;
+    hipLaunchKernelGGL(gc_finish_kernel, dim3(1), dim3(256), 0, st, slots, used, scale, max_norm, norm);
+    return hipGetLastError() == hipSuccess ? 0 : cdae_fail("grad_norm finish launch failed");
+}
+
+int cdae_grad_clip(const void* const* in, const long* n, const int* types, void* const* out, const int* out_types, int count, double scale, double max_norm,
+                   float* norm, void* ws, size_t ws_bytes, void* stream) {
+    if (check_list("grad_clip: a list of device tensors with sizes >= 0 and types 0 (bf16), 1 (fp16), 2 (fp32)", in, n, types, count)) return -1;
+    if (check_list("grad_clip: outputs beside every input, types 0 (bf16), 1 (fp16), 2 (fp32)", (const void* const*)out, n, out_types, count)) return -1;
+    if (!norm || !ws || ws_bytes < cdae_grad_workspace_bytes()) return cdae_fail("grad_clip: norm[2] and a workspace of cdae_grad_workspace_bytes() required");
+    if (!(max_norm >= 0.0)) return cdae_fail("grad_clip: max_norm must be a number >= 0 (infinity: nothing is clipped)");
+    if (const int rc = check_overlap(in, n, types, out, out_types, count))
+        return cdae_fail(rc == 1 ? "grad_clip: two outputs share memory, or an output shares memory with a gradient other than its own" : "grad_clip: out of host memory");
+    hipStream_t st = (hipStream_t)stream;
+    double* slots = (double*)ws;
+    const int used = launch_norm(in, n, types, count, slots, st);
+    if (used < 0) return -1;
+    if (!used) {
+        hipLaunchKernelGGL(gc_finish_kernel, dim3(1), dim3(256), 0, st, slots, 0, scale, max_norm, norm);
+        return hipGetLastError() == hipSuccess ? 0 : cdae_fail("grad_clip finish launch failed");
+    }
+    int at = 0;
+    while (at < count) {
+        GcTab t;
+        long chunks;
+        at = fill(t, in, n, types, out, out_types, count, at, chunks);
+        if (!t.count) break;
+        const long blocks = chunks < 2 * GC_BLOCKS ? chunks : 2 * GC_BLOCKS;
+        hipLaunchKernelGGL(gc_scale_kernel, dim3((unsigned)blocks), dim3(256), 0, st, t, chunks, slots, used, scale, max_norm, norm);
+        if (hipGetLastError() != hipSuccess) return cdae_fail("grad_clip launch failed");
+    }
+    return 0;
+}
+
+}  // extern "C"

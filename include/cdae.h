@@ -461,6 +461,10 @@ int cdae_adamw_ema(float* p, const float* g, float* m, float* v, float* ema, lon
    mean of the all-reduced sum, train_util.py:111-118, without a pass of its own) */
 int cdae_adamw_ema_multi(float* p, const float* g, float* m, float* v, float* const* emas, const double* ema_rates, int n_ema, long n, double lr,
                          double beta1, double beta2, double eps, double weight_decay, int step, double grad_scale, void* stream);
+/* cdae_adamw_ema_multi with the gradient's factor read from DEVICE memory (the second value of cdae_grad_norm's norm[2]): clipping by the global norm
+   without a pass of its own over the gradients and without a host synchronisation */
+int cdae_adamw_ema_factor(float* p, const float* g, float* m, float* v, float* const* emas, const double* ema_rates, int n_ema, long n, double lr,
+                          double beta1, double beta2, double eps, double weight_decay, int step, const float* factor, void* stream);
 int cdae_sqsum(const float* x, long n, double* out, void* stream);                                            /* grad-norm, train_util.py:299-303 */
 int cdae_mse_rows(const float* a, const float* b, float* out, int N, long per, void* stream);               /* mean_flat((a-b)^2), gaussian_diffusion.py:847 */
 int cdae_mse_rows_bwd(const float* a, const float* b, const float* gout, float* db, int N, long per, void* stream);
@@ -564,6 +568,49 @@ int cdae_im2col3x3_16(const void* x, void* y, int N, int H, int W, int C, void* 
 int cdae_wprep_all_m16(const float* flat, const void* desc, int nw, int total_tiles, long base, unsigned short* f_hi, unsigned short* f_lo,
                        unsigned short* b_hi, unsigned short* b_lo, unsigned short* kf_hi, unsigned short* kf_lo, unsigned short* kb_hi,
                        unsigned short* kb_lo, const float* w_scales, void* stream);
+
+/* ---- a feed-forward block on rows: linear layers with an activation, the norms around the block, and the step that trains it.
+   Row types: 0 bf16, 1 fp16, 2 fp32 (the linear layers: 0 or 1).  Nothing is kept between calls; workspaces belong to one call at a time. */
+/* y[M][N] = act(x[M][K] @ w[N][K]^T + bias) + res on 16-bit rows, fp32 accumulation, one rounding (lin16.hip).  Operands of one 16-bit type at any
+   pitch >= a row and any alignment; bias [N] and res [M][N] may be NULL.  act: 0 none, 1 SiLU, 3 ReLU, 5 GELU, 6 GELU in its tanh form.  z (may be
+   NULL; for the backward) receives the pre-activation as fp16 whatever dt is, clamped to +-65504.
+   cdae_lin16_bwd: dx = dz @ w, dw = dz^T @ x, dbias = column sums of dz with dz = dy * act'(z) (rounded to the rows' type as an operand of the
+   products; the sums take it unrounded); each result may be NULL.  The gradient of res is dy itself. */
+enum { CDAE_LIN16_FWD = 0, CDAE_LIN16_BWD = 1 };
+size_t cdae_lin16_workspace_bytes(int op, int M, int N, int K);
+int cdae_lin16_fwd(const void* x, long ldx, const void* w, long ldw, const void* bias, const void* res, long ldres, void* y, long ldy, void* z, long ldz, int M,
+                   int N, int K, int act, int dt, void* ws, size_t ws_bytes, void* stream);
+int cdae_lin16_bwd(const void* dy, long lddy, const void* x, long ldx, const void* w, long ldw, const void* z, long ldz, void* dx, long lddx, void* dw, long lddw,
+                   void* dbias, int M, int N, int K, int act, int dt, void* ws, size_t ws_bytes, void* stream);
+/* The norms before and after a block with its gate and residual scale (resnorm.hip), rows [B * T][C], 1 <= C <= 8192:
+       r = x + alpha * gate o post(f),    u = pre(r) o (1 + scale) + shift
+   post and pre: layer norms (layer = 1) or rms norms (0) with weight and bias (w1, b1 / w2, b2: each may be NULL), or absent.  f may be NULL: then
+   r = x, and r is not written.  gate, scale, shift: a vector for each sample (a row pitch ld_*), or one for all samples (shared_* = 1), or NULL; fp32
+   (vec32 = 1) or the rows' type; w and b likewise (w32).  r, u and the gradients of rows are dense; x, f, dr, du have pitches.
+   Backward: dr and du in (either may be NULL); every output may be NULL.  dgate, dscale and dshift are dense, [B][C], or [C] for a shared vector. */
+typedef struct cdae_resnorm {
+    int B, T, C, dt, layer, post, pre, vec32, w32, shared_gate, shared_scale, shared_shift;
+    float alpha, eps;
+    const void *x, *f, *gate, *scale, *shift, *w1, *b1, *w2, *b2;
+    long ld_x, ld_f, ld_gate, ld_scale, ld_shift;
+    void *r, *u;
+    const void *dr, *du;
+    long ld_dr, ld_du;
+    void *dx, *df, *dgate, *dscale, *dshift, *dw1, *db1, *dw2, *db2;
+    float* ws; size_t ws_bytes;
+} cdae_resnorm;
+size_t cdae_resnorm_workspace_bytes(int B, int T, int C);
+int cdae_resnorm_fwd(const cdae_resnorm* p, void* stream);
+int cdae_resnorm_bwd(const cdae_resnorm* p, void* stream);
+/* The global norm of `count` gradients (HOST arrays of device pointers, sizes and types; elements dense) and clipping by it (gradclip.hip):
+       n = |scale| sqrt(sum of squares),   factor = scale * min(1, max_norm / (n + 1e-6)),   out = g * factor
+   norm[2] (device, fp32) receives n and the factor.  Sums are fp64 in a fixed order.  out[i] may be in[i] itself (in place) and of another type;
+   outputs that share memory otherwise are refused.  A norm that is not finite reaches the outputs as 0 * g or NaN and is for the caller to look at. */
+size_t cdae_grad_workspace_bytes(void);
+int cdae_grad_norm(const void* const* in, const long* n, const int* types, int count, double scale, double max_norm, float* norm, void* ws, size_t ws_bytes,
+                   void* stream);
+int cdae_grad_clip(const void* const* in, const long* n, const int* types, void* const* out, const int* out_types, int count, double scale, double max_norm,
+                   float* norm, void* ws, size_t ws_bytes, void* stream);
 
 /* ---- opt-in profiler (prof.hip): HIP events on the launch stream around every launch of a kernel family */
 int cdae_prof_enable(int on);

@@ -1,0 +1,113 @@
+"""Refusals and sizes of the feed-forward block's entry points that are decided on the host, before any launch (no GPU)."""
+import array
+import ctypes
+
+import pytest
+import torch
+
+from causaldiffae_amd import CdaeError, ops_block
+from causaldiffae_amd._lib import ResNorm, lib
+
+PTR = 0x10000          # never followed: every call below is refused first
+
+
+def refused(rc, word):
+    assert rc == -1 and word in lib.cdae_last_error().decode(), (rc, lib.cdae_last_error())
+
+
+def test_workspace_sizes():
+    assert lib.cdae_lin16_workspace_bytes(0, 0, 8, 8) == 0 and lib.cdae_lin16_workspace_bytes(7, 8, 8, 8) == 0
+    for op in (0, 1):
+        assert lib.cdae_lin16_workspace_bytes(op, 1, 1, 1) > 0
+        assert lib.cdae_lin16_workspace_bytes(op, 1 << 20, 4096, 4096) >= (1 << 20) * 4096 * 2         # (sizes beyond 32 bits)
+    assert lib.cdae_resnorm_workspace_bytes(1, 1, 8193) == 0 and lib.cdae_resnorm_workspace_bytes(0, 1, 8) == 0
+    assert lib.cdae_resnorm_workspace_bytes(1, 1, 8192) >= 4 * 4 * 8192
+    assert lib.cdae_grad_workspace_bytes() >= 8 * 1024
+
+
+def test_linear_refusals():
+    def fwd(M=4, N=8, K=8, act=0, dt=0, ldx=8, ldw=8, ldy=8, x=PTR, y=PTR, ws=PTR, ws_bytes=1 << 30):
+        return lib.cdae_lin16_fwd(x, ldx, PTR, ldw, None, None, 0, y, ldy, None, 0, M, N, K, act, dt, ws, ws_bytes, None)
+
+    def bwd(M=4, N=8, K=8, act=0, dt=0, dy=PTR, x=PTR, w=PTR, z=None, dx=PTR, dw=PTR, ws_bytes=1 << 30):
+        return lib.cdae_lin16_bwd(dy, 8, x, 8, w, 8, z, 8, dx, 8, dw, 8, None, M, N, K, act, dt, PTR, ws_bytes, None)
+
+    for kw in (dict(M=-1), dict(N=0), dict(K=0)):
+        refused(fwd(**kw), "required")
+        refused(bwd(**kw), "required")
+    refused(fwd(dt=2), "type")
+    refused(bwd(dt=3), "type")
+    for a in (2, 4, 7, -1):
+        refused(fwd(act=a), "activation")
+        refused(bwd(act=a), "activation")
+    for kw in (dict(ldx=7), dict(ldw=7), dict(ldy=7), dict(x=None), dict(y=None)):
+        refused(fwd(**kw), "pitches")
+    refused(fwd(ws_bytes=16), "workspace")
+    refused(fwd(ws=None), "workspace")
+    refused(bwd(ws_bytes=16), "workspace")
+    refused(bwd(M=0), "no rows")
+    refused(bwd(dy=None), "dy")
+    refused(bwd(act=1), "z with an activation")
+    refused(bwd(w=None), "w for dx")
+    refused(bwd(x=None), "x for dw")
+    assert fwd(M=0) == 0
+
+
+def test_norm_refusals():
+    def args(**kw):
+        p = ResNorm()
+        d = dict(B=2, T=3, C=8, dt=0, layer=1, pre=1, alpha=1.0, eps=1e-5, x=PTR, ld_x=8, u=PTR, du=PTR, ld_du=8, ws=PTR, ws_bytes=1 << 20)
+        for k, v in {**d, **kw}.items():
+            setattr(p, k, v)
+        return ctypes.byref(p)
+
+    both = (lib.cdae_resnorm_fwd, lib.cdae_resnorm_bwd)
+    for f in both:
+        for kw in (dict(B=0), dict(T=0), dict(C=0), dict(C=8193)):
+            refused(f(args(**kw), None), "required")
+        refused(f(args(B=1 << 20, T=1 << 20), None), "rows")
+        refused(f(args(dt=3), None), "type")
+        refused(f(args(x=None), None), "required")
+        refused(f(args(gate=PTR), None), "block output")
+        refused(f(args(pre=0, f=PTR, r=PTR, scale=PTR), None), "pre norm")
+        refused(f(args(f=PTR, r=PTR, w1=PTR), None), "post norm")
+        refused(f(args(eps=-1.0), None), "eps")
+        refused(f(args(eps=float("nan")), None), "eps")
+    refused(lib.cdae_resnorm_fwd(args(u=None), None), "u with a pre norm")
+    refused(lib.cdae_resnorm_fwd(args(f=PTR), None), "r with a block output")
+    refused(lib.cdae_resnorm_bwd(args(du=None), None), "gradient of r or of u")
+    refused(lib.cdae_resnorm_bwd(args(df=PTR), None), "not there")
+    refused(lib.cdae_resnorm_bwd(args(dscale=PTR), None), "not there")
+    refused(lib.cdae_resnorm_bwd(args(ws_bytes=16), None), "workspace")
+    refused(lib.cdae_resnorm_bwd(args(B=1 << 18, C=8192, T=1, ws_bytes=1 << 60), None), "samples")
+
+
+def test_grad_refusals():
+    def call(ptrs=(PTR,), sizes=(16,), types=(2,), outs=None, out_types=None, max_norm=1.0, norm=PTR, ws_bytes=1 << 20):
+        keep = [array.array("Q", ptrs), array.array("q", sizes), array.array("i", types), array.array("Q", outs or ptrs), array.array("i", out_types or types)]
+        p, n, t, o, ot = (k.buffer_info()[0] for k in keep)
+        return (lib.cdae_grad_norm(p, n, t, len(ptrs), 1.0, max_norm, norm, PTR, ws_bytes, None),
+                lib.cdae_grad_clip(p, n, t, o, ot, len(ptrs), 1.0, max_norm, norm, PTR, ws_bytes, None))
+
+    for kw in (dict(sizes=(-1,)), dict(ptrs=(0,)), dict(types=(3,)), dict(types=(-1,)), dict(norm=None), dict(ws_bytes=8), dict(max_norm=-1.0), dict(max_norm=float("nan"))):
+        assert call(**kw) == (-1, -1), kw
+
+    def clip(**kw):
+        keep = {k: array.array(c, kw[k]) for k, c in (("ptrs", "Q"), ("sizes", "q"), ("types", "i"), ("outs", "Q"), ("out_types", "i"))}
+        a = {k: v.buffer_info()[0] for k, v in keep.items()}
+        return lib.cdae_grad_clip(a["ptrs"], a["sizes"], a["types"], a["outs"], a["out_types"], len(kw["ptrs"]), 1.0, 1.0, PTR, PTR, 1 << 20, None)
+
+    far = 0x900000
+    # the same tensor twice, an overlapping pair, outputs that overlap, an output over another gradient, an output of another size over its own gradient
+    for ptrs, sizes, types, outs, out_types in (
+            ((PTR, PTR), (16, 16), (2, 2), (PTR, PTR), (2, 2)), ((PTR, PTR + 32), (16, 16), (2, 2), (PTR, PTR + 32), (2, 2)),
+            ((PTR, far), (16, 16), (2, 2), (PTR, PTR + 60), (2, 2)), ((PTR, far), (16, 16), (2, 2), (far, PTR), (2, 2)), ((PTR,), (16,), (0,), (PTR,), (2,)),
+            ((PTR,), (16,), (2,), (PTR + 4,), (2,))):
+        refused(clip(ptrs=ptrs, sizes=sizes, types=types, outs=outs, out_types=out_types), "shares memory" if len(set(outs)) == len(outs) else "share memory")
+
+
+def test_host_tensors_are_refused():
+    x = torch.zeros(4, 8, dtype=torch.bfloat16)
+    for call in (lambda: ops_block.linear_act(x, x), lambda: ops_block.residual_norm(x, x), lambda: ops_block.grad_norm([x]), lambda: ops_block.clip_grad_norm_([x], 1.0)):
+        with pytest.raises(CdaeError):
+            call()

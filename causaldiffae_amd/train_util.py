@@ -16,7 +16,7 @@ import numpy as np
 import torch as th
 import torch.distributed as dist
 
-from . import dist_util, logger, ops
+from . import dist_util, logger, ops, ops_block
 from ._lib import check, lib, ptr, stream
 from .resample import LossAwareSampler, UniformSampler
 
@@ -231,19 +231,25 @@ class FusedAdamWEMA:
         check(lib.cdae_sqsum(ptr(self.flat.grad), self.flat.numel, ptr(self._sq), stream()))
         return float(self._sq.item()) * grad_scale * grad_scale
 
-    def step(self, lr=None, grad_scale=1.0):
+    def step(self, lr=None, grad_scale=1.0, max_norm=None):
         """One AdamW step on `grad_scale * gradient` + every EMA rate, ONE kernel over the flat buffers (groups of four rates per launch;
-        only the first launch of a step moves the weights)."""
+        only the first launch of a step moves the weights).  max_norm: the gradient is clipped to that global norm (after grad_scale): one
+        pass that reads it for the norm, whose factor the optimizer kernel then takes from device memory — the gradient is not written."""
         import ctypes
+        if max_norm is not None:
+            ops.side_join()              # (the norm reads what ops' weight-gradient stream writes)
+            norm = ops_block.grad_factor([self.flat.grad], max_norm, grad_scale)
         self.t += 1
         f = self.flat
         ops.side_join()                  # backward() already joined ops' weight-gradient stream; a caller that wrote gradients otherwise has not
         n = len(self.ema)
         emas = (ctypes.c_void_p * max(1, min(4, n)))(*[e.data_ptr() for e in self.ema[:4]])
         rates = (ctypes.c_double * max(1, min(4, n)))(*self.ema_rates[:4])
-        check(lib.cdae_adamw_ema_multi(ptr(f.flat), ptr(f.grad), ptr(self.m), ptr(self.v), emas, rates, min(4, n), f.numel,
-                                       self.lr if lr is None else lr, self.betas[0], self.betas[1], self.eps, self.weight_decay,
-                                       self.t, grad_scale, stream()))
+        hyper = (self.lr if lr is None else lr, self.betas[0], self.betas[1], self.eps, self.weight_decay, self.t)
+        if max_norm is None:
+            check(lib.cdae_adamw_ema_multi(ptr(f.flat), ptr(f.grad), ptr(self.m), ptr(self.v), emas, rates, min(4, n), f.numel, *hyper, grad_scale, stream()))
+        else:
+            check(lib.cdae_adamw_ema_factor(ptr(f.flat), ptr(f.grad), ptr(self.m), ptr(self.v), emas, rates, min(4, n), f.numel, *hyper, norm.data_ptr() + 4, stream()))
         for rate, e in zip(self.ema_rates[4:], self.ema[4:]):          # (more than four rates: never seen in the reference's scripts)
             e.mul_(rate).add_(f.flat, alpha=1 - rate)
         ops.bump_weight_epoch()          # parameter storage was rewritten by a raw kernel: cached pre-split weight planes are stale
@@ -294,7 +300,10 @@ class TrainLoop:
     def __init__(self, *, model, diffusion, data, batch_size, microbatch, lr, ema_rate, log_interval, save_interval,
                  resume_checkpoint, use_fp16=False, fp16_scale_growth=1e-3, schedule_sampler=None, weight_decay=0.0,
                  lr_anneal_steps=0, rep_cond=False, n_vars=None, causal_modeling=False, flow_based=False, in_channels=3,
-                 masking=False, bucket_mb=64, use_graph=False, run_ahead=1, throttle_poll_s=0.0005):
+                 masking=False, bucket_mb=64, use_graph=False, run_ahead=1, throttle_poll_s=0.0005, grad_clip=0.0):
+        if not grad_clip >= 0.0:
+            raise ValueError(f"grad_clip is the largest global gradient norm of a step, or 0 for none (got {grad_clip})")
+        self.grad_clip = float(grad_clip)
         if use_fp16:       # reduced-precision torso; fp32 master weights are the only weights, bf16 gradients need no loss scaling
             model.convert_to_fp16()        # marks THIS model (the mode is scoped to its forward / backward, not process-wide)
         self.model, self.diffusion, self.data = model, diffusion, data
@@ -455,7 +464,7 @@ class TrainLoop:
 
     def optimize_normal(self):
         self._anneal_lr()
-        self.opt.step(self._lr, grad_scale=getattr(self, "_grad_scale", 1.0))
+        self.opt.step(self._lr, grad_scale=getattr(self, "_grad_scale", 1.0), max_norm=self.grad_clip or None)
         self._throttle()
 
     def _throttle(self):

@@ -3,7 +3,7 @@
 `model_and_diffusion_defaults()` plus data_dir / schedule_sampler / lr / weight_decay / lr_anneal_steps / batch_size /
 microbatch / ema_rate / log_interval / save_interval / resume_checkpoint / use_fp16 / fp16_scale_growth / rep_cond /
 n_vars / causal_modeling / flow_based / in_channels / masking.  Additions: --log_dir (the reference edits a hard-coded
-path in the source), --split, --host_feed (default: the dataset shard lives in HBM and batches are assembled on the GPU).
+path in the source), --split, --grad_clip (largest global gradient norm of a step, 0: none), --host_feed (default: the dataset shard lives in HBM and batches are assembled on the GPU).
 
     python scripts/image_train.py --data_dir ../datasets/pendulum --image_size 96 --in_channels 4 --n_vars 4 \
         --rep_cond True --causal_modeling True --batch_size 32 --log_dir ../results/pendulum/causaldiffae
@@ -29,7 +29,7 @@ def create_argparser():
                     microbatch=-1, ema_rate="0.9999", log_interval=10, save_interval=5000, resume_checkpoint="",
                     use_fp16=False, fp16_scale_growth=1e-3, rep_cond=False, n_vars=None, causal_modeling=False,
                     flow_based=False, in_channels=3, masking=False,
-                    log_dir="", split="train", host_feed=False)
+                    log_dir="", split="train", host_feed=False, grad_clip=0.0)
     defaults.update(model_and_diffusion_defaults())
     parser = argparse.ArgumentParser()
     add_dict_to_argparser(parser, defaults)
@@ -56,7 +56,7 @@ def main():
               resume_checkpoint=args.resume_checkpoint, use_fp16=args.use_fp16, fp16_scale_growth=args.fp16_scale_growth,
               schedule_sampler=schedule_sampler, weight_decay=args.weight_decay, lr_anneal_steps=args.lr_anneal_steps,
               rep_cond=args.rep_cond, n_vars=args.n_vars, causal_modeling=args.causal_modeling, flow_based=args.flow_based,
-              in_channels=args.in_channels, masking=args.masking).run_loop()
+              in_channels=args.in_channels, masking=args.masking, grad_clip=args.grad_clip).run_loop()
 
 
 if __name__ == "__main__":

@@ -619,3 +619,67 @@ def test_block_in_two_graphs():
         for w, o in zip(want, outs):
             assert all(torch.equal(p, q) for p, q in zip(w, o)), k
 
+
+# ----------------------------------------------------------------------------- clipping inside the optimizer step
+def test_optimizer_step_clips():
+    """FusedAdamWEMA.step(max_norm) is the step whose grad_scale is the factor of the definition, and leaves the gradients as they are"""
+    from causaldiffae_amd.nn import Linear
+    from causaldiffae_amd.train_util import FusedAdamWEMA
+
+    def build():
+        torch.manual_seed(3)
+        m = torch.nn.Sequential(Linear(33, 50), Linear(50, 7)).to(DEV)
+        opt = FusedAdamWEMA(m, lr=1e-2, weight_decay=0.1, ema_rates=(0.9, 0.99))
+        opt.zero_grad()
+        for i, p in enumerate(m.parameters()):
+            p.grad.copy_(rnd(i, *p.shape))
+        return m, opt
+
+    (m1, a), (m2, b) = build(), build()
+    n = exact_norm([p.grad for p in m1.parameters()], 0.5)
+    for max_norm in (n / 3, n * 3, math.inf):
+        keep = a.flat.grad.clone()
+        a.step(grad_scale=0.5, max_norm=max_norm)
+        factor = blk().grad_factor([b.flat.grad], max_norm, 0.5)
+        assert abs(float(factor[1]) - 0.5 * min(1.0, max_norm / (n + 1e-6))) <= 2 * u
+        b.step(grad_scale=float(factor[1]))
+        assert torch.equal(keep, a.flat.grad)
+        for p, q in ((a.flat.flat, b.flat.flat), (a.m, b.m), (a.v, b.v), *zip(a.ema, b.ema)):
+            assert torch.equal(p, q)
+
+
+def test_train_loop_clips():
+    """TrainLoop(grad_clip): with a bound far above the norm a step is bit for bit the step without one; with a small bound the first moments are the
+    clipped gradient's (beta1 = 0.9: m = 0.1 factor g), whose norm is the bound"""
+    from improved_diffusion import script_util as su
+    from improved_diffusion.train_util import TrainLoop
+    data = iter([(torch.rand(2, 1, 32, 32) * 2 - 1, {"y": torch.tensor([1, 7])})] * 3)
+    batch, cond = next(data)
+
+    def loop(clip):
+        torch.manual_seed(0)
+        cfg = dict(image_size=32, in_channels=1, num_channels=32, num_res_blocks=1, class_cond=True, timestep_respacing="")
+        model, diff = su.create_model_and_diffusion(**{**su.model_and_diffusion_defaults(), **cfg})
+        model.to(DEV)
+        with torch.no_grad():                       # (the zero-initialised output convs would leave most gradients at zero)
+            for p in model.parameters():
+                p.add_(0.02 * torch.randn(p.shape, device=DEV))
+        lp = TrainLoop(model=model, diffusion=diff, data=data, batch_size=2, microbatch=-1, lr=1e-3, ema_rate="0.99", log_interval=10 ** 9, save_interval=10 ** 9,
+                       resume_checkpoint="", grad_clip=clip)
+        torch.manual_seed(5)
+        lp.forward_backward(batch, cond)
+        return lp
+
+    a, b, c = loop(0.0), loop(1e6), loop(0.125)
+    b.opt.flat.grad.copy_(a.opt.flat.grad)          # (two backward passes need not agree to the bit)
+    n = exact_norm([a.opt.flat.grad])
+    assert 0.125 < n < 1e6
+    for lp in (a, b, c):
+        lp.optimize_normal()
+    assert torch.equal(a.opt.flat.flat, b.opt.flat.flat) and torch.equal(a.opt.m, b.opt.m)
+    g = c.opt.flat.grad.double()
+    nc = float(g.norm())
+    within("m", c.opt.m, 0.1 * g * (0.125 / (nc + 1e-6)), 8 * u * g.abs() * (0.125 / nc))
+    assert exact_norm([c.opt.m]) == pytest.approx(0.0125, rel=1e-4)
+    with pytest.raises(ValueError):
+        TrainLoop(model=None, diffusion=None, data=None, batch_size=1, microbatch=1, lr=0.0, ema_rate="0", log_interval=1, save_interval=1, resume_checkpoint="", grad_clip=-1.0)

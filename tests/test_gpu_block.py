@@ -152,6 +152,34 @@ def test_linear_act_partial_gradients():
     assert torch.equal(g, dy)
 
 
+def test_linear_act_without_bias():
+    x, w, res, dy = rnd(1, 2, 25, 40, dtype=F16), rnd(2, 24, 40, dtype=F16, scale=0.2), rnd(3, 2, 25, 24, dtype=F16), rnd(4, 2, 25, 24, dtype=F16)
+    check_linear(x, w, None, res, "gelu_tanh", dy)
+    x, w, res = (t.detach() for t in (x, w, res))
+    with torch.no_grad():
+        y = blk().linear_act(x.requires_grad_(True), w, None, res, "gelu_tanh")
+    assert not y.requires_grad and torch.equal(y, blk().linear_act(x, w, None, res, "gelu_tanh").detach())
+
+
+def test_first_derivatives_only():
+    """a gradient of a gradient raises instead of being zero"""
+    x, w = rnd(1, 6, 16, dtype=BF16).requires_grad_(True), rnd(2, 16, 16, dtype=BF16).requires_grad_(True)
+    for y in (blk().linear_act(x, w, act="silu"), blk().residual_norm(x, x, pre=w[0])[1]):
+        (g,) = torch.autograd.grad(y.float().sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="first derivatives"):
+            g.float().sum().backward()
+
+
+def test_accumulating_backward():
+    """.backward() twice into the leaves' .grad, an input that occurs twice, and outputs of which one is not used"""
+    x, w = rnd(1, 12, 16, dtype=F32).requires_grad_(True), (1 + rnd(2, 16)).requires_grad_(True)
+    r, uu = blk().residual_norm(x, x, alpha=2.0, pre=w, kind="rms")
+    (3 * r).sum().backward()
+    assert torch.equal(x.grad, torch.full_like(x, 9.0)) and w.grad is not None and not w.grad.any()
+    blk().residual_norm(x, x, alpha=2.0, pre=w, kind="rms")[0].sum().backward()
+    assert torch.equal(x.grad, torch.full_like(x, 12.0))
+
+
 def test_linear_act_rows_do_not_mix():
     """a row that is not finite stays alone, at a size with rows, columns and k outside full tiles"""
     x, w = rnd(1, 131, 72, dtype=BF16), rnd(2, 133, 72, dtype=BF16, scale=0.1)

@@ -16,7 +16,14 @@
 // call's own inputs is kept for it, and r enters it unrounded as in the forward.
 //
 // Bound: HBM (four tensors of rows forward, six backward; ~20 / 60 operations a value).  A row lives in the registers of TPR threads, 8 values
-// each, so it is read once whatever the number of reductions; a row's sums are a butterfly inside a wave and a pass through LDS across waves.
+// each, so it is read once whatever the number of reductions.  What makes it run at the memory's rate:
+//   * loads without branches around them: a branch makes the compiler wait for each load at its end (the first form, with a branch for a row's
+//     ragged end in every load, took 18.9 us for 8192 x 384 bf16 rows forward).  The last thread's 8 values are the row's LAST 8: they overlap its
+//     neighbour's, count once in sums and are written twice with the same value.  Rows past a block's end repeat its last row the same way;
+//   * the next row is requested before this one is worked on, and the vectors are folded to four (forward) or three (backward) per chunk of rows:
+//     r = x + n1 (g w1) + g b1,   u = n2 (w2 (1 + s)) + (b2 (1 + s) + t);
+//   * sums inside a wave on the lane-permute instructions (no LDS), across waves through LDS with ONE barrier: a wave hands over (mean, sum of
+//     squares about it), which combine exactly, so a layer norm needs no second round and no difference of large sums.
 // All arithmetic and all sums are fp32; a result is rounded once, when it is written.
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -30,243 +37,390 @@ namespace {
 constexpr int RN_V = 8;                          // values of a row in one thread's registers
 constexpr int RN_MAX_C = 8192;                   // 1024 threads x 8
 constexpr long RN_MAX_GRID = 1 << 20;            // (a launch holds fewer than 2^32 threads: more rows than this are walked by the same blocks)
-constexpr long RN_MAX_FOLD = 1 << 23;            // samples x 64-column blocks of a backward call (the same bound)
+constexpr long RN_MAX_FOLD = 1 << 21;            // samples x 32-column blocks of a backward call (the same bound)
 
 constexpr int RN_SUMS = 7;                       // of a sample: g A1, g A2, (1 + s) A3, (1 + s) A4, and the gradients of g, s, t
 
 struct RnArgs {
     cdae_resnorm p;
-    int nch, rows_per_chunk;                     // backward: chunks of a sample, rows of a chunk
+    int nch, rows_per_chunk;                     // chunks of a sample, rows of a chunk
 };
 
-// sums of a (and b) over the TPR threads of a row
-template <int TPR, int NV>
-__device__ __forceinline__ void row_sum(float (&a)[NV], float* sh) {
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+// sum over aligned groups of N lanes, in every lane of the group
+template <int N>
+__device__ __forceinline__ float lane_sum(float v) {
+    v += dpp<0xb1>(v);                                                    // quad_perm 1 0 3 2
+    if constexpr (N >= 4) v += dpp<0x4e>(v);                              // quad_perm 2 3 0 1
+    if constexpr (N >= 8) v += dpp<0x141>(v);                             // the other quad of 8 lanes (half mirror)
+    if constexpr (N >= 16) v += dpp<0x140>(v);                            // the other half of 16 lanes (mirror)
+    if constexpr (N >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+        v = __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+    }
+    if constexpr (N >= 64) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+        v = __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+    }
+    return v;
+}
+
+// The sums of a row over its TPR threads.  Across waves: two LDS buffers in turn, so that one barrier separates a sum's writes from its reads and
+// the buffer of the sum before last is free again (whoever has passed this barrier has read it).
+template <int TPR>
+struct RowSum {
+    static constexpr int L = TPR < 64 ? TPR : 64, W = TPR / 64;           // (W: waves of a row; a row of up to 64 threads needs no LDS)
+    float* sh;
+    int turn = 0;
+    __device__ explicit RowSum(float* buf) : sh(buf) {}
+    template <int NV>
+    __device__ __forceinline__ void add(float (&a)[NV]) {
 #pragma unroll
-    for (int o = (TPR < 64 ? TPR : 64) / 2; o > 0; o >>= 1)
+        for (int i = 0; i < NV; ++i) a[i] = lane_sum<L>(a[i]);
+        if constexpr (W > 1) {
+            float* b = sh + (turn ^= 1) * (2 * W);
+            if ((threadIdx.x & 63) == 0)
 #pragma unroll
-        for (int i = 0; i < NV; ++i) a[i] += __shfl_xor(a[i], o);
-    if constexpr (TPR > 64) {
-        constexpr int W = TPR / 64;
-        const int wave = threadIdx.x >> 6;
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0)
+                for (int i = 0; i < NV; ++i) b[(threadIdx.x >> 6) * 2 + i] = a[i];
+            __syncthreads();
 #pragma unroll
-            for (int i = 0; i < NV; ++i) sh[wave * NV + i] = a[i];
-        __syncthreads();
-        const int w0 = wave / W * W;
+            for (int i = 0; i < NV; ++i) {
+                a[i] = 0.f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
+                for (int w = 0; w < W; ++w) a[i] += b[w * 2 + i];
+            }
+        }
+    }
+    // n = the normalised row, -> 1 / sqrt(mean square + eps)
+    __device__ __forceinline__ float normalise(const float (&v)[RN_V], float (&n)[RN_V], int skip, int end, int C, int layer, float inv_c, float eps) {
+        float m = 0.f, q[1] = {0.f};
+        if (!layer) {
+#pragma unroll
+            for (int e = 0; e < RN_V; ++e) q[0] += e >= skip && e < end ? v[e] * v[e] : 0.f;
+            add<1>(q);
+        } else {
             float s = 0.f;
 #pragma unroll
-            for (int w = 0; w < W; ++w) s += sh[(w0 + w) * NV + i];
-            a[i] = s;
+            for (int e = 0; e < RN_V; ++e) s += e >= skip && e < end ? v[e] : 0.f;
+            if constexpr (W <= 1) {
+                m = lane_sum<L>(s) * inv_c;
+#pragma unroll
+                for (int e = 0; e < RN_V; ++e) { const float d = v[e] - m; q[0] += e >= skip && e < end ? d * d : 0.f; }
+                q[0] = lane_sum<L>(q[0]);
+            } else {
+                const int wave = threadIdx.x >> 6;
+                auto count = [&](int w) { const int k = C - w * 64 * RN_V; return (float)(k < 0 ? 0 : k < 64 * RN_V ? k : 64 * RN_V); };
+                const float mine = count(wave);
+                const float mw = mine > 0.f ? lane_sum<64>(s) / mine : 0.f;
+#pragma unroll
+                for (int e = 0; e < RN_V; ++e) { const float d = v[e] - mw; q[0] += e >= skip && e < end ? d * d : 0.f; }
+                q[0] = lane_sum<64>(q[0]);
+                float* b = sh + (turn ^= 1) * (2 * W);
+                if ((threadIdx.x & 63) == 0) { b[wave * 2] = mw; b[wave * 2 + 1] = q[0]; }
+                __syncthreads();
+                float sum = 0.f;
+#pragma unroll
+                for (int w = 0; w < W; ++w) sum = fmaf(count(w), b[2 * w], sum);
+                m = sum * inv_c;
+                q[0] = 0.f;
+#pragma unroll
+                for (int w = 0; w < W; ++w) { const float d = b[2 * w] - m; q[0] += fmaf(count(w) * d, d, b[2 * w + 1]); }
+            }
+        }
+        const float i = 1.f / sqrtf(q[0] * inv_c + eps);
+#pragma unroll
+        for (int e = 0; e < RN_V; ++e) n[e] = (v[e] - m) * i;
+        return i;
+    }
+};
+
+// A thread's 8 columns.  Rows of 8 values and more: columns c0 .. c0 + 7 with c0 at most C - 8, of which the first `skip` belong to the thread
+// before (skip >= 8: all; such a thread repeats the last 8).  Shorter rows (SMALL): one thread's, with C values; the other threads repeat them.
+template <bool SMALL>
+struct Cols {
+    int c0, skip, end, C;                        // (the thread's own values: [skip, end) of its 8)
+    __device__ Cols(int lane, int C_) : C(C_) {
+        const int want = lane * RN_V;
+        c0 = SMALL ? 0 : want < C - RN_V ? want : C - RN_V;
+        skip = SMALL ? (lane ? RN_V : 0) : want - c0;
+        end = SMALL ? C : RN_V;
+    }
+    template <class T>
+    __device__ __forceinline__ Pack<T, RN_V> raw(const T* __restrict__ p) const {
+        if constexpr (SMALL) {
+            Pack<T, RN_V> v;
+#pragma unroll
+            for (int e = 0; e < RN_V; ++e) v.v[e] = p[e < C ? e : C - 1];
+            return v;
+        } else {
+            return *reinterpret_cast<const Pack<T, RN_V>*>(p + c0);
         }
     }
-}
-
-// n = normalised v (n values present), i = 1 / sqrt(mean square + eps); two passes over registers: the squares are of centred values
-template <int TPR>
-__device__ __forceinline__ float normalise(const float (&v)[RN_V], float (&n)[RN_V], int have, int layer, float inv_c, float eps, float* sh) {
-    float m = 0.f;
-    if (layer) {
-        float s[1] = {0.f};
+    template <class T>
+    __device__ __forceinline__ void put(T* __restrict__ p, const float (&v)[RN_V]) const {
+        if constexpr (SMALL) {
 #pragma unroll
-        for (int e = 0; e < RN_V; ++e) s[0] += v[e];              // (absent values are zero)
-        row_sum<TPR, 1>(s, sh);
-        m = s[0] * inv_c;
+            for (int e = 0; e < RN_V; ++e) if (e < C) st1(p[e], v[e]);
+        } else {
+            stv<T, RN_V>(p + c0, v);
+        }
     }
-    float q[1] = {0.f};
+    template <class T>
+    __device__ __forceinline__ void vec(const void* p, long off, int is32, float (&o)[RN_V]) const {
+        if (is32) open(raw(reinterpret_cast<const float*>(p) + off), o);
+        else open(raw(reinterpret_cast<const T*>(p) + off), o);
+    }
+    // values that are absent read as zero (SMALL) or count elsewhere (skip)
+    template <class T>
+    __device__ __forceinline__ void open(const Pack<T, RN_V>& r, float (&o)[RN_V]) const {
 #pragma unroll
-    for (int e = 0; e < RN_V; ++e) { n[e] = e < have ? v[e] - m : 0.f; q[0] = fmaf(n[e], n[e], q[0]); }
-    row_sum<TPR, 1>(q, sh);
-    const float i = 1.f / sqrtf(q[0] * inv_c + eps);
-#pragma unroll
-    for (int e = 0; e < RN_V; ++e) n[e] *= i;
-    return i;
-}
+        for (int e = 0; e < RN_V; ++e) o[e] = SMALL && e >= C ? 0.f : ld1(r.v[e]);
+    }
+};
 
-struct RnCol { float g[RN_V], w1[RN_V], b1[RN_V], w2[RN_V], b2[RN_V], s[RN_V], t[RN_V]; };
-
-template <class T>
-__device__ __forceinline__ void load_cols(const cdae_resnorm& p, long b, int c0, int have, RnCol& k, bool shift) {
+// the vectors folded: r = x + n1 gw + gb,  u = n2 sw + sb
+template <class T, bool SMALL>
+__device__ __forceinline__ void fold_cols(const cdae_resnorm& p, long b, const Cols<SMALL>& k, float (&gw)[RN_V], float (&gb)[RN_V], float (&sw)[RN_V], float (&sb)[RN_V]) {
+    float t[RN_V];
 #pragma unroll
-    for (int e = 0; e < RN_V; ++e) { k.g[e] = p.alpha; k.w1[e] = 1.f; k.b1[e] = 0.f; k.w2[e] = 1.f; k.b2[e] = 0.f; k.s[e] = 1.f; k.t[e] = 0.f; }
+    for (int e = 0; e < RN_V; ++e) { gw[e] = p.alpha; gb[e] = 0.f; sw[e] = 1.f; sb[e] = 0.f; }
     if (p.gate) {
-        ldv_n2<T, RN_V>(p.gate, (p.shared_gate ? 0 : b * p.ld_gate) + c0, p.vec32, have, k.g);
+        k.template vec<T>(p.gate, p.shared_gate ? 0 : b * p.ld_gate, p.vec32, t);
 #pragma unroll
-        for (int e = 0; e < RN_V; ++e) k.g[e] *= p.alpha;
+        for (int e = 0; e < RN_V; ++e) gw[e] *= t[e];
     }
-    if (p.w1) ldv_n2<T, RN_V>(p.w1, c0, p.w32, have, k.w1);
-    if (p.b1) ldv_n2<T, RN_V>(p.b1, c0, p.w32, have, k.b1);
-    if (p.w2) ldv_n2<T, RN_V>(p.w2, c0, p.w32, have, k.w2);
-    if (p.b2) ldv_n2<T, RN_V>(p.b2, c0, p.w32, have, k.b2);
+    if (p.b1) {
+        k.template vec<T>(p.b1, 0, p.w32, t);
+#pragma unroll
+        for (int e = 0; e < RN_V; ++e) gb[e] = gw[e] * t[e];
+    }
+    if (p.w1) {
+        k.template vec<T>(p.w1, 0, p.w32, t);
+#pragma unroll
+        for (int e = 0; e < RN_V; ++e) gw[e] *= t[e];
+    }
     if (p.scale) {
-        ldv_n2<T, RN_V>(p.scale, (p.shared_scale ? 0 : b * p.ld_scale) + c0, p.vec32, have, k.s);
+        k.template vec<T>(p.scale, p.shared_scale ? 0 : b * p.ld_scale, p.vec32, t);
 #pragma unroll
-        for (int e = 0; e < RN_V; ++e) k.s[e] += 1.f;
+        for (int e = 0; e < RN_V; ++e) sw[e] += t[e];
     }
-    if (shift && p.shift) ldv_n2<T, RN_V>(p.shift, (p.shared_shift ? 0 : b * p.ld_shift) + c0, p.vec32, have, k.t);
+    if (p.b2) {
+        k.template vec<T>(p.b2, 0, p.w32, t);
+#pragma unroll
+        for (int e = 0; e < RN_V; ++e) sb[e] = sw[e] * t[e];
+    }
+    if (p.w2) {
+        k.template vec<T>(p.w2, 0, p.w32, t);
+#pragma unroll
+        for (int e = 0; e < RN_V; ++e) sw[e] *= t[e];
+    }
+    if (p.shift) {
+        k.template vec<T>(p.shift, p.shared_shift ? 0 : b * p.ld_shift, p.vec32, t);
+#pragma unroll
+        for (int e = 0; e < RN_V; ++e) sb[e] += t[e];
+    }
 }
 
-template <class T, int TPR>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rn_fwd_kernel(const RnArgs a) {
-    constexpr int BLOCK = TPR < 256 ? 256 : TPR, RPB = BLOCK / TPR;
-    __shared__ float sh[16];
+// threads of a block: four waves of rows that need no LDS, or one row
+constexpr int block_of(int tpr) { return tpr <= 64 ? 256 : tpr; }
+
+// A group of TPR threads walks one chunk of a sample's rows.
+template <class T, int TPR, bool SMALL>
+__global__ __launch_bounds__(block_of(TPR)) void rn_fwd_kernel(const RnArgs a) {
+    constexpr int GROUPS = block_of(TPR) / TPR;
+    __shared__ float sh[TPR > 64 ? 4 * (TPR / 64) : 1];
     const cdae_resnorm& p = a.p;
-    const int c0 = (threadIdx.x & (TPR - 1)) * RN_V;
-    const int have = p.C - c0 < 0 ? 0 : p.C - c0 < RN_V ? p.C - c0 : RN_V;
+    const Cols<SMALL> k(threadIdx.x & (TPR - 1), p.C);
     const float inv_c = 1.f / (float)p.C;
-    const long M = (long)p.B * p.T;
-    for (long row0 = (long)blockIdx.x * RPB; row0 < M; row0 += (long)gridDim.x * RPB) {
-    const long row = row0 + threadIdx.x / TPR;
-    const bool live = row < M;
-    const int mine = live ? have : 0;
-    const long rr = live ? row : M - 1;                          // (a row past the end computes the last one's and writes nothing)
-    RnCol k;
-    load_cols<T>(p, rr / p.T, c0, have, k, true);
-    float r[RN_V];
-    ldv_n<T, RN_V>(reinterpret_cast<const T*>(p.x) + rr * p.ld_x + c0, have, r);
-    if (p.f) {
-        float f[RN_V], n[RN_V];
-        ldv_n<T, RN_V>(reinterpret_cast<const T*>(p.f) + rr * p.ld_f + c0, have, f);
-        if (p.post) {
-            normalise<TPR>(f, n, have, p.layer, inv_c, p.eps, sh);
+    const long chunks = (long)p.B * a.nch;
+    for (long c = (long)blockIdx.x * GROUPS + threadIdx.x / TPR; c < chunks; c += (long)gridDim.x * GROUPS) {      // (one group a block where there are barriers)
+        RowSum<TPR> rows(sh);
+        const long b = c / a.nch;
+        const int t0 = (int)(c - b * a.nch) * a.rows_per_chunk, t1 = t0 + a.rows_per_chunk < p.T ? t0 + a.rows_per_chunk : p.T;
+        float gw[RN_V], gb[RN_V], sw[RN_V], sb[RN_V];
+        const T* X = reinterpret_cast<const T*>(p.x) + (b * p.T) * p.ld_x;
+        const T* F = reinterpret_cast<const T*>(p.f);
+        if (F) F += b * p.T * p.ld_f;
+        const long out = b * p.T * p.C;
+        Pack<T, RN_V> xr = k.raw(X + t0 * p.ld_x), fr = k.raw(F ? F + t0 * p.ld_f : X + t0 * p.ld_x);
+        fold_cols<T, SMALL>(p, b, k, gw, gb, sw, sb);
+        for (int t = t0; t < t1; ++t) {
+            const int next = t + 1 < t1 ? t + 1 : t;
+            float r[RN_V], n[RN_V];
+            k.open(xr, r);
+            k.open(fr, n);
+            xr = k.raw(X + next * p.ld_x);
+            if (F) {
+                fr = k.raw(F + next * p.ld_f);
+                if (p.post) {
+                    float f[RN_V];
 #pragma unroll
-            for (int e = 0; e < RN_V; ++e) f[e] = fmaf(n[e], k.w1[e], k.b1[e]);
+                    for (int e = 0; e < RN_V; ++e) f[e] = n[e];
+                    rows.normalise(f, n, k.skip, k.end, p.C, p.layer, inv_c, p.eps);
+                }
+#pragma unroll
+                for (int e = 0; e < RN_V; ++e) r[e] = fmaf(n[e], gw[e], r[e]) + gb[e];
+                k.put(reinterpret_cast<T*>(p.r) + out + (long)t * p.C, r);
+            }
+            if (p.pre) {
+                rows.normalise(r, n, k.skip, k.end, p.C, p.layer, inv_c, p.eps);
+#pragma unroll
+                for (int e = 0; e < RN_V; ++e) n[e] = fmaf(n[e], sw[e], sb[e]);
+                k.put(reinterpret_cast<T*>(p.u) + out + (long)t * p.C, n);
+            }
         }
-#pragma unroll
-        for (int e = 0; e < RN_V; ++e) r[e] = e < have ? fmaf(k.g[e], f[e], r[e]) : 0.f;
-        stv_n<T, RN_V>(reinterpret_cast<T*>(p.r) + rr * p.C + c0, mine, r);
-    }
-    if (p.pre) {
-        float n[RN_V];
-        normalise<TPR>(r, n, have, p.layer, inv_c, p.eps, sh);
-#pragma unroll
-        for (int e = 0; e < RN_V; ++e) n[e] = fmaf(fmaf(n[e], k.w2[e], k.b2[e]), k.s[e], k.t[e]);
-        stv_n<T, RN_V>(reinterpret_cast<T*>(p.u) + rr * p.C + c0, mine, n);
-    }
     }
 }
 
-// One block: rows [r0, r1) of one sample.  Leaves dx, df, and the four column sums of its rows in part[chunk][4][C].
-template <class T, int TPR>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rn_bwd_kernel(const RnArgs a) {
-    constexpr int BLOCK = TPR < 256 ? 256 : TPR, RPB = BLOCK / TPR;
-    __shared__ float sh[32];
-    __shared__ float cols[RPB > 1 ? RPB * TPR * RN_V : 1];
+// One block: rows [t0, t1) of one sample, its groups of TPR threads in turn.  Leaves dx, df, and the four column sums of its rows in part[chunk][4][C].
+template <class T, int TPR, bool SMALL>
+__global__ __launch_bounds__(block_of(TPR)) void rn_bwd_kernel(const RnArgs a) {
+    constexpr int BLOCK = block_of(TPR), GROUPS = BLOCK / TPR;
+    __shared__ float sh[TPR > 64 ? 4 * (TPR / 64) : 1];
+    __shared__ float cols[GROUPS > 1 ? GROUPS * TPR * RN_V : 1];
     const cdae_resnorm& p = a.p;
     const int lane = threadIdx.x & (TPR - 1), grp = threadIdx.x / TPR;
-    const int c0 = lane * RN_V;
-    const int have = p.C - c0 < 0 ? 0 : p.C - c0 < RN_V ? p.C - c0 : RN_V;
+    const Cols<SMALL> k(lane, p.C);
+    RowSum<TPR> rows(sh);
     const float inv_c = 1.f / (float)p.C;
-    const int b = blockIdx.x / a.nch, ch = blockIdx.x - b * a.nch;
-    const long first = (long)b * p.T;
+    const long b = blockIdx.x / a.nch;
+    const int ch = blockIdx.x - (int)b * a.nch;
     const int t0 = ch * a.rows_per_chunk, t1 = t0 + a.rows_per_chunk < p.T ? t0 + a.rows_per_chunk : p.T;
-    RnCol k;
-    load_cols<T>(p, b, c0, have, k, false);
+    const T* X = reinterpret_cast<const T*>(p.x) + b * p.T * p.ld_x;
+    const T* F = reinterpret_cast<const T*>(p.f);
+    const T* R = reinterpret_cast<const T*>(p.dr);
+    const T* U = reinterpret_cast<const T*>(p.du);
+    if (F) F += b * p.T * p.ld_f;
+    if (R) R += b * p.T * p.ld_dr;
+    if (U) U += b * p.T * p.ld_du;
+    const long out = b * p.T * p.C;
+    // (a tensor that is absent is read as x and not used)
+    const T* const Fs = F ? F : X; const T* const Rs = R ? R : X; const T* const Us = U ? U : X;
+    const long lf = F ? p.ld_f : p.ld_x, lr = R ? p.ld_dr : p.ld_x, lu = U ? p.ld_du : p.ld_x;
+    auto row_of = [&](int t) { return t + grp < t1 ? t + grp : t1 - 1; };
+    int t = row_of(t0);
+    constexpr bool AHEAD = TPR < 1024;                            // (1024 threads have 128 registers each: none left for the next row)
+    Pack<T, RN_V> xr = k.raw(X + t * p.ld_x), fr = k.raw(Fs + t * lf), rr = k.raw(Rs + t * lr), ur = k.raw(Us + t * lu);
+    float gw[RN_V], gb[RN_V], sw[RN_V], sb[RN_V];
+    fold_cols<T, SMALL>(p, b, k, gw, gb, sw, sb);
     float A[4][RN_V];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int e = 0; e < RN_V; ++e) A[j][e] = 0.f;
-    for (int tb = t0; tb < t1; tb += RPB) {                       // (the trip count is the block's: its barriers are met by every thread)
-        const bool live = tb + grp < t1;
-        const long row = first + (live ? tb + grp : t1 - 1);
-        const int mine = live ? have : 0;
-        float r[RN_V], n1[RN_V], D[RN_V], f[RN_V];
-        float i1 = 0.f;
-        ldv_n<T, RN_V>(reinterpret_cast<const T*>(p.x) + row * p.ld_x + c0, have, r);
+    for (int tb = t0; tb < t1; tb += GROUPS) {                    // (the trip count is the block's: its barriers are met by every thread)
+        const float live = tb + grp < t1 ? 1.f : 0.f;
+        t = row_of(tb);
+        const int next = row_of(tb + GROUPS < t1 ? tb + GROUPS : tb);
+        float r[RN_V], n1[RN_V], n2[RN_V], D[RN_V], h[RN_V];
+        if (!AHEAD) { xr = k.raw(X + t * p.ld_x); fr = k.raw(Fs + t * lf); rr = k.raw(Rs + t * lr); ur = k.raw(Us + t * lu); }
+        k.open(xr, r);
+        k.open(fr, n1);
+        k.open(rr, D);
+        k.open(ur, h);
+        if (AHEAD) { xr = k.raw(X + next * p.ld_x); fr = k.raw(Fs + next * lf); rr = k.raw(Rs + next * lr); ur = k.raw(Us + next * lu); }
+        float i1 = 1.f;
+        if (!R)
 #pragma unroll
-        for (int e = 0; e < RN_V; ++e) { D[e] = 0.f; n1[e] = 0.f; }
-        if (p.dr) ldv_n<T, RN_V>(reinterpret_cast<const T*>(p.dr) + row * p.ld_dr + c0, mine, D);
-        if (p.f) {
-            ldv_n<T, RN_V>(reinterpret_cast<const T*>(p.f) + row * p.ld_f + c0, have, f);
-            if (p.post) i1 = normalise<TPR>(f, n1, have, p.layer, inv_c, p.eps, sh);
-            else
+            for (int e = 0; e < RN_V; ++e) D[e] = 0.f;
+        if (F) {
+            if (p.post) {
+                float f[RN_V];
 #pragma unroll
-                for (int e = 0; e < RN_V; ++e) n1[e] = f[e];
+                for (int e = 0; e < RN_V; ++e) f[e] = n1[e];
+                i1 = rows.normalise(f, n1, k.skip, k.end, p.C, p.layer, inv_c, p.eps);
+            }
 #pragma unroll
-            for (int e = 0; e < RN_V; ++e) r[e] = e < have ? fmaf(k.g[e], fmaf(n1[e], k.w1[e], k.b1[e]), r[e]) : 0.f;
+            for (int e = 0; e < RN_V; ++e) r[e] = fmaf(n1[e], gw[e], r[e]) + gb[e];
         }
-        if (p.pre && p.du) {
-            float U[RN_V], n2[RN_V];
-            ldv_n<T, RN_V>(reinterpret_cast<const T*>(p.du) + row * p.ld_du + c0, mine, U);
-            const float i2 = normalise<TPR>(r, n2, have, p.layer, inv_c, p.eps, sh);
+        if (U) {
+            const float i2 = rows.normalise(r, n2, k.skip, k.end, p.C, p.layer, inv_c, p.eps);
             float s[2] = {0.f, 0.f};
 #pragma unroll
             for (int e = 0; e < RN_V; ++e) {
-                A[2][e] = fmaf(U[e], n2[e], A[2][e]);
-                A[3][e] += U[e];
-                U[e] = U[e] * k.s[e] * k.w2[e];
-                s[0] = fmaf(U[e], n2[e], s[0]);
-                s[1] += U[e];
+                A[2][e] = fmaf(live * h[e], n2[e], A[2][e]);
+                A[3][e] = fmaf(live, h[e], A[3][e]);
+                h[e] *= sw[e];
+                if (e >= k.skip && e < k.end) { s[0] = fmaf(h[e], n2[e], s[0]); s[1] += h[e]; }
             }
-            row_sum<TPR, 2>(s, sh);
+            rows.add(s);
             const float m1 = s[0] * inv_c, m0 = p.layer ? s[1] * inv_c : 0.f;
 #pragma unroll
-            for (int e = 0; e < RN_V; ++e) D[e] += e < mine ? i2 * (U[e] - m0 - n2[e] * m1) : 0.f;
+            for (int e = 0; e < RN_V; ++e) D[e] = fmaf(i2, h[e] - m0 - n2[e] * m1, D[e]);
         }
-        if (p.dx) stv_n<T, RN_V>(reinterpret_cast<T*>(p.dx) + row * p.C + c0, mine, D);
-        if (p.f) {
+        if (p.dx) k.put(reinterpret_cast<T*>(p.dx) + out + (long)t * p.C, D);
+        if (F) {
             float s[2] = {0.f, 0.f};
 #pragma unroll
             for (int e = 0; e < RN_V; ++e) {
-                A[0][e] = fmaf(D[e], n1[e], A[0][e]);
-                A[1][e] += D[e];
-                D[e] = D[e] * k.g[e] * k.w1[e];
-                s[0] = fmaf(D[e], n1[e], s[0]);
-                s[1] += D[e];
+                A[0][e] = fmaf(live * D[e], n1[e], A[0][e]);
+                A[1][e] = fmaf(live, D[e], A[1][e]);
+                D[e] *= gw[e];
+                if (e >= k.skip && e < k.end) { s[0] = fmaf(D[e], n1[e], s[0]); s[1] += D[e]; }
             }
-            if (p.post && p.df) {
-                row_sum<TPR, 2>(s, sh);
-                const float m1 = s[0] * inv_c, m0 = p.layer ? s[1] * inv_c : 0.f;
+            if (p.df) {
+                if (p.post) {
+                    rows.add(s);
+                    const float m1 = s[0] * inv_c, m0 = p.layer ? s[1] * inv_c : 0.f;
 #pragma unroll
-                for (int e = 0; e < RN_V; ++e) D[e] = i1 * (D[e] - m0 - n1[e] * m1);
+                    for (int e = 0; e < RN_V; ++e) D[e] = i1 * (D[e] - m0 - n1[e] * m1);
+                }
+                k.put(reinterpret_cast<T*>(p.df) + out + (long)t * p.C, D);
             }
-            if (p.df) stv_n<T, RN_V>(reinterpret_cast<T*>(p.df) + row * p.C + c0, mine, D);
         }
     }
     float* part = p.ws + (long)blockIdx.x * 4 * p.C;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        if constexpr (RPB > 1) {                                  // the block's row groups, added in a fixed order
+        if constexpr (GROUPS > 1) {                               // the block's groups, added in a fixed order
             __syncthreads();
 #pragma unroll
-            for (int e = 0; e < RN_V; ++e) cols[(grp * TPR + lane) * RN_V + e] = A[j][e];
+            for (int e = 0; e < RN_V; ++e) if (SMALL ? e < p.C && !lane : true) cols[grp * TPR * RN_V + k.c0 + e] = A[j][e];
             __syncthreads();
             for (int c = threadIdx.x; c < p.C; c += BLOCK) {
                 float s = 0.f;
-                for (int g = 0; g < RPB; ++g) s += cols[g * TPR * RN_V + c];
+#pragma unroll 4
+                for (int g = 0; g < GROUPS; ++g) s += cols[g * TPR * RN_V + c];
                 part[j * p.C + c] = s;
             }
         } else {
-            stv_n<float, RN_V>(part + j * p.C + c0, have, A[j]);
+            k.put(part + j * p.C, A[j]);
         }
     }
 }
 
 // The column sums of each sample from its chunks, and from them the gradients of gate, scale and shift; what the samples
-// share goes to sums[b][7][C].  A block: 64 columns x 4 lanes of chunks.
+// share goes to sums[b][7][C].  A block: 32 columns (one line of a chunk's row) x 32 lanes of chunks.
 template <class T>
-__global__ __launch_bounds__(256) void rn_fold_kernel(const RnArgs a, float* __restrict__ sums) {
+__global__ __launch_bounds__(1024) void rn_fold_kernel(const RnArgs a, float* __restrict__ sums) {
     const cdae_resnorm& p = a.p;
-    const int ncb = (p.C + 63) / 64, b = blockIdx.x / ncb;
-    const int c = (blockIdx.x - b * ncb) * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6;
-    __shared__ float sh[4][4][64];
+    const int ncb = (p.C + 31) / 32;
+    const long b = blockIdx.x / ncb;
+    const int cl = threadIdx.x & 31, q = threadIdx.x >> 5, c = (int)(blockIdx.x - b * ncb) * 32 + cl;
+    __shared__ float sh[4][32][33];
     float A[4] = {0.f, 0.f, 0.f, 0.f};
-    if (c < p.C)
-        for (int ch = q; ch < a.nch; ch += 4) {
-            const float* part = p.ws + ((long)b * a.nch + ch) * 4 * p.C + c;
+    const float* part = p.ws + b * a.nch * 4 * p.C + (c < p.C ? c : p.C - 1);
+#pragma unroll 4
+    for (int ch = q; ch < a.nch; ch += 32) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) A[j] += part[(long)j * p.C];
-        }
+        for (int j = 0; j < 4; ++j) A[j] += part[((long)ch * 4 + j) * p.C];
+    }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sh[q][j][threadIdx.x & 63] = A[j];
+    for (int j = 0; j < 4; ++j) sh[j][q][cl] = A[j];
+    __syncthreads();
+    if (q < 4) {                                                          // wave pair q of a block adds sum q, in order
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) s += sh[q][i][cl];
+        sh[q][0][cl] = s;
+    }
     __syncthreads();
     if (q || c >= p.C) return;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) A[j] = (sh[0][j][threadIdx.x] + sh[1][j][threadIdx.x]) + (sh[2][j][threadIdx.x] + sh[3][j][threadIdx.x]);
+    for (int j = 0; j < 4; ++j) A[j] = sh[j][0][cl];
     auto vec = [&](const void* v, long off, int is32, float none) { return !v ? none : is32 ? ((const float*)v)[off] : ld1(((const T*)v)[off]); };
     const float g = vec(p.gate, (p.shared_gate ? 0 : b * p.ld_gate) + c, p.vec32, 1.f) * p.alpha, s1 = 1.f + vec(p.scale, (p.shared_scale ? 0 : b * p.ld_scale) + c, p.vec32, 0.f);
     const float w1 = vec(p.w1, c, p.w32, 1.f), b1 = vec(p.b1, c, p.w32, 0.f), w2 = vec(p.w2, c, p.w32, 1.f), b2 = vec(p.b2, c, p.w32, 0.f);
@@ -279,18 +433,26 @@ __global__ __launch_bounds__(256) void rn_fold_kernel(const RnArgs a, float* __r
     for (int j = 0; j < RN_SUMS; ++j) sums[((long)b * RN_SUMS + j) * p.C + c] = o[j];
 }
 
-// what all samples share: grid y picks one of the seven sums
+// what all samples share: grid y picks one of the seven sums; 32 columns x 8 lanes of samples
 template <class T>
 __global__ __launch_bounds__(256) void rn_shared_kernel(const RnArgs a, const float* __restrict__ sums) {
     const cdae_resnorm& p = a.p;
-    const int c = blockIdx.x * 256 + threadIdx.x, j = blockIdx.y;
+    const int cl = threadIdx.x & 31, q = threadIdx.x >> 5, c = blockIdx.x * 32 + cl, j = blockIdx.y;
+    __shared__ float sh[8][32];
     void* const dst[RN_SUMS] = {p.dw1, p.db1, p.dw2, p.db2, p.shared_gate ? p.dgate : nullptr, p.shared_scale ? p.dscale : nullptr, p.shared_shift ? p.dshift : nullptr};
     void* out = nullptr;
 #pragma unroll
     for (int i = 0; i < RN_SUMS; ++i) if (i == j) out = dst[i];
-    if (!out || c >= p.C) return;
+    if (!out) return;                                                     // (block-uniform)
     float s = 0.f;
-    for (int b = 0; b < p.B; ++b) s += sums[((long)b * RN_SUMS + j) * p.C + c];
+    const float* at = sums + (long)j * p.C + (c < p.C ? c : p.C - 1);
+#pragma unroll 4
+    for (int b = q; b < p.B; b += 8) s += at[(long)b * RN_SUMS * p.C];
+    sh[q][cl] = s;
+    __syncthreads();
+    if (q || c >= p.C) return;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) s += sh[i][cl];
     st2<T>(out, c, j < 4 ? p.w32 : p.vec32, s);
 }
 
@@ -300,13 +462,18 @@ int threads_per_row(int C) {
     return t < 8 ? 8 : t;
 }
 
-// chunks of a sample: about 1024 blocks in all, at least one pass of a block's row groups each
+// Backward: chunks of a sample for about 1024 blocks in all (four a CU), a multiple of the block's groups of rows each.  Forward: a group's chunk,
+// for about 16 waves a CU; longer chunks read the vectors less often, but past 16 rows that is nothing.
 void chunks_of(int B, int T, int C, int& nch, int& rows) {
-    const int tpr = threads_per_row(C), rpb = tpr < 256 ? 256 / tpr : 1;
-    long want = (1024 + B - 1) / B;
+    const int tpr = threads_per_row(C), groups = block_of(tpr) / tpr;
+    const long want = (1024 + B - 1) / B;
     rows = (int)((T + want - 1) / want);
-    if (rows < rpb) rows = rpb;
-    rows = (rows + rpb - 1) / rpb * rpb;
+    rows = (rows + groups - 1) / groups * groups;
+    nch = (T + rows - 1) / rows;
+}
+void fwd_chunks(int B, int T, int C, int& nch, int& rows) {
+    const long tpr = threads_per_row(C), r = (long)B * T * tpr / 64 / 4096;
+    rows = r < 1 ? 1 : r > 16 ? 16 : (int)r;
     nch = (T + rows - 1) / rows;
 }
 
@@ -322,25 +489,27 @@ int check(const cdae_resnorm* p) {
     return 0;
 }
 
-#define RN_TPR(CALL)                          \
-    switch (threads_per_row(p->C)) {          \
-        case 8: { CALL(8); break; }           \
-        case 16: { CALL(16); break; }         \
-        case 32: { CALL(32); break; }         \
-        case 64: { CALL(64); break; }         \
-        case 128: { CALL(128); break; }       \
-        case 256: { CALL(256); break; }       \
-        case 512: { CALL(512); break; }       \
-        default: { CALL(1024); break; }       \
+#define RN_TPR(CALL)                                    \
+    if (p->C < RN_V) { CALL(8, true); }                 \
+    else switch (threads_per_row(p->C)) {               \
+        case 8: { CALL(8, false); break; }              \
+        case 16: { CALL(16, false); break; }            \
+        case 32: { CALL(32, false); break; }            \
+        case 64: { CALL(64, false); break; }            \
+        case 128: { CALL(128, false); break; }          \
+        case 256: { CALL(256, false); break; }          \
+        case 512: { CALL(512, false); break; }          \
+        default: { CALL(1024, false); break; }          \
     }
 
 template <class T>
 void fwd(const cdae_resnorm* p, hipStream_t st) {
     RnArgs a;
-    a.p = *p; a.nch = a.rows_per_chunk = 0;
-    const long M = (long)p->B * p->T;
-#define RN_CALL(N) { constexpr int BL = N < 256 ? 256 : N; const long g = (M + BL / N - 1) / (BL / N); \
-                     hipLaunchKernelGGL((rn_fwd_kernel<T, N>), dim3((unsigned)(g < RN_MAX_GRID ? g : RN_MAX_GRID)), dim3(BL), 0, st, a); }
+    a.p = *p;
+    fwd_chunks(p->B, p->T, p->C, a.nch, a.rows_per_chunk);
+    const long chunks = (long)p->B * a.nch;
+#define RN_CALL(N, S) { constexpr int G = block_of(N) / N; const long g = (chunks + G - 1) / G; \
+                        hipLaunchKernelGGL((rn_fwd_kernel<T, N, S>), dim3((unsigned)(g < RN_MAX_GRID ? g : RN_MAX_GRID)), dim3(block_of(N)), 0, st, a); }
     RN_TPR(RN_CALL)
 #undef RN_CALL
 }
@@ -350,13 +519,13 @@ void bwd(const cdae_resnorm* p, hipStream_t st) {
     a.p = *p;
     chunks_of(p->B, p->T, p->C, a.nch, a.rows_per_chunk);
     float* sums = p->ws + (long)p->B * a.nch * 4 * p->C;
-#define RN_CALL(N) { constexpr int BL = N < 256 ? 256 : N; hipLaunchKernelGGL((rn_bwd_kernel<T, N>), dim3((unsigned)((long)p->B * a.nch)), dim3(BL), 0, st, a); }
+#define RN_CALL(N, S) hipLaunchKernelGGL((rn_bwd_kernel<T, N, S>), dim3((unsigned)((long)p->B * a.nch)), dim3(block_of(N)), 0, st, a)
     RN_TPR(RN_CALL)
 #undef RN_CALL
     if (!(p->dgate || p->dscale || p->dshift || p->dw1 || p->db1 || p->dw2 || p->db2)) return;
-    hipLaunchKernelGGL((rn_fold_kernel<T>), dim3((unsigned)((p->C + 63) / 64 * (long)p->B)), dim3(256), 0, st, a, sums);
+    hipLaunchKernelGGL((rn_fold_kernel<T>), dim3((unsigned)((p->C + 31) / 32 * (long)p->B)), dim3(1024), 0, st, a, sums);
     if (p->dw1 || p->db1 || p->dw2 || p->db2 || (p->dgate && p->shared_gate) || (p->dscale && p->shared_scale) || (p->dshift && p->shared_shift))
-        hipLaunchKernelGGL((rn_shared_kernel<T>), dim3((p->C + 255) / 256, RN_SUMS), dim3(256), 0, st, a, sums);
+        hipLaunchKernelGGL((rn_shared_kernel<T>), dim3((p->C + 31) / 32, RN_SUMS), dim3(256), 0, st, a, sums);
 }
 
 }  // namespace
@@ -382,7 +551,7 @@ int cdae_resnorm_fwd(const cdae_resnorm* p, void* stream) {
 
 int cdae_resnorm_bwd(const cdae_resnorm* p, void* stream) {
     if (check(p)) return -1;
-    if ((long)p->B * ((p->C + 63) / 64) > RN_MAX_FOLD) return cdae_fail("resnorm_bwd: at most 2^23 / ceil(C / 64) samples");
+    if ((long)p->B * ((p->C + 31) / 32) > RN_MAX_FOLD) return cdae_fail("resnorm_bwd: at most 2^21 / ceil(C / 32) samples");
     if (!p->dr && !p->du) return cdae_fail("resnorm_bwd: the gradient of r or of u required");
     if (p->du && !p->pre) return cdae_fail("resnorm_bwd: the gradient of u without a pre norm");
     if (!p->f && (p->df || p->dgate || p->dw1 || p->db1)) return cdae_fail("resnorm_bwd: gradients of a block output that is not there");

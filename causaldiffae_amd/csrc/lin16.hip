@@ -26,22 +26,37 @@ enum { L_NONE = 0, L_SILU = 1, L_RELU = 3, L_GELU = 5, L_GELU_TANH = 6 };      /
 
 __device__ __attribute__((aligned(16))) unsigned g_zero_lin16[4] = {0u, 0u, 0u, 0u};
 
+// Activations and slopes for results of 16 bits: a few steps of fp32 from the exact value, on the exp2 and reciprocal instructions.
+//   logistic(a) = 1 / (1 + 2^(-a log2 e)): where 2^t overflows the reciprocal is 0, the limit.
+//   The normal distribution function after Abramowitz & Stegun, Handbook of Mathematical Functions, 7.1.26 (absolute error 1.5e-7, and its
+//   exp(-z^2 / 2) is the density the slope needs): 15 instructions where the library's erf takes about 40, and the epilogue is bound by them
+//   (12.6 million values of a 8192 x 1536 result: 40 instructions a value are 13 us of all vector units).
+__device__ __forceinline__ float logistic(float a) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * a)); }
+__device__ __forceinline__ float normal_cdf(float z, float& e) {
+    const float x = fabsf(z) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.f));
+    e = __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z);                                       // exp(-z^2 / 2)
+    const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+    const float tail = 0.5f * p * e;                                                                 // of the side that z points to
+    return z < 0.f ? tail : 1.f - tail;
+}
+__device__ __forceinline__ float gelu_tanh_arg(float z) { return 1.5957691216057308f * z * fmaf(0.044715f * z, z, 1.f); }      // 0.5 (1 + tanh a) = logistic(2 a)
+
 __device__ __forceinline__ float act_fwd(float z, int act) {
     switch (act) {
-        case L_SILU: return z * cdae_sigmoid(z);
+        case L_SILU: return z * logistic(z);
         case L_RELU: return z > 0.f ? z : (z != z ? z : 0.f);
-        case L_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-        case L_GELU_TANH: return z * cdae_sigmoid(1.5957691216057308f * fmaf(0.044715f * z * z, z, z));      // 0.5 (1 + tanh a) = sigmoid(2 a)
+        case L_GELU: { float e; return z * normal_cdf(z, e); }
+        case L_GELU_TANH: return z * logistic(gelu_tanh_arg(z));
         default: return z;
     }
 }
 __device__ __forceinline__ float act_slope(float z, int act) {
     switch (act) {
-        case L_SILU: { const float s = cdae_sigmoid(z); return s * fmaf(z, 1.f - s, 1.f); }
-        case L_RELU: return z > 0.f ? 1.f : 0.f;
-        case L_GELU: return fmaf(0.3989422804014327f * z, expf(-0.5f * z * z), 0.5f * (1.f + erff(z * 0.70710678118654752f)));
+        case L_SILU: { const float s = logistic(z); return s * fmaf(z, 1.f - s, 1.f); }
+        case L_RELU: return z > 0.f ? 1.f : (z != z ? z : 0.f);
+        case L_GELU: { float e; const float c = normal_cdf(z, e); return fmaf(0.3989422804014327f * z, e, c); }
         case L_GELU_TANH: {
-            const float s = cdae_sigmoid(1.5957691216057308f * fmaf(0.044715f * z * z, z, z));
+            const float s = logistic(gelu_tanh_arg(z));
             return s * fmaf(z * (1.f - s), 1.5957691216057308f * fmaf(0.134145f * z, z, 1.f), 1.f);
         }
         default: return 1.f;
@@ -74,14 +89,10 @@ template <> struct Mfma<F16> {
 
 // v[0..n) of row m from column n0: bias, activation, residual, rounding
 template <class T, int V>
-__device__ __forceinline__ void finish_row(const LinArgs& p, long m, int n0, int n, float (&v)[V]) {
+__device__ __forceinline__ void finish_row(const LinArgs& p, long m, int n0, int n, float (&v)[V], const float (&bias)[V]) {
     if (n <= 0) return;
-    float t[V];
-    if (p.bias) {
-        ldv_n<T, V>(reinterpret_cast<const T*>(p.bias) + n0, n, t);
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] += t[i];
-    }
+    for (int i = 0; i < V; ++i) v[i] += bias[i];
     if (p.z) {
         _Float16* zp = p.z + m * p.ldz + n0;
         Pack<F16, V> k;
@@ -96,57 +107,111 @@ __device__ __forceinline__ void finish_row(const LinArgs& p, long m, int n0, int
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] = act_fwd(v[i], p.act);
     if (p.res) {
+        float t[V];
         ldv_n<T, V>(reinterpret_cast<const T*>(p.res) + m * p.ldres + n0, n, t);
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] += t[i];
     }
     stv_n<T, V>(reinterpret_cast<T*>(p.y) + m * p.ldy + n0, n, v);
 }
+template <class T, int V>
+__device__ __forceinline__ void load_bias(const LinArgs& p, int n0, int n, float (&b)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) b[i] = 0.f;
+    if (p.bias && n > 0) ldv_n<T, V>(reinterpret_cast<const T*>(p.bias) + n0, n, b);
+}
 
-// 128 x 128 tile, four waves of 64 x 64, 32 k a step
-template <class T, bool AMC, bool BMC>
-__global__ __launch_bounds__(256, 2) void lin_tile_kernel(const LinArgs p) {
-    constexpr int OPB = 128 * 64, STAGE = 2 * OPB;                       // bytes of one operand's step
-    __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * STAGE];
+// LDS-DMA with a scalar base and a 32-bit offset a lane: advancing along k costs no vector instruction
+__device__ __forceinline__ void lds_dma16_s(const void* base, unsigned off, unsigned lds_dst) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_dst), "v"(off), "s"(base) : "memory", "m0");
+}
+
+// One BM x BN tile of the result (and one range of k): WM x WN waves, 64 k a stage.
+//   * stages arrive by LDS-DMA in two slots; the request for stage S + 2 goes out when the second half of stage S begins, one barrier a stage;
+//   * the fragments of the next 32 k are read from LDS while these 32 k run on the matrix cores (two register sets), so no product waits for LDS;
+//   * operand images: KC, rows of 128 bytes (whole cache lines: with 64-byte rows each line was fetched twice, 581 us for 16384 x 8192 x 2048 where
+//     the MC x MC product of the same size took 458) whose 16-byte piece j lies at j ^ f(row); MC, 128-column planes of 256-byte k rows whose piece j lies
+//     at j ^ 2 g(k row), read through the transpose read.  f, g spread the rows that one read touches over all banks; the permutation is applied to
+//     the global address of the DMA lane;
+//   * the operands are swapped in the instruction (B in the A slot): a lane's four accumulators are four consecutive columns of one row;
+//   * blocks that run on one XCD (block number mod 8) take neighbouring tiles, 8 rows of tiles at a time: an operand's panel is read from HBM once an XCD.
+template <class T, bool AMC, bool BMC, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, 2) void lin_tile_kernel(const LinArgs p) {
+    constexpr int TM = BM / WM, TN = BN / WN, FA = TM / 16, FB = TN / 16;                 // a wave's part and its fragments
+    constexpr int AB = BM * 128, STAGE = (BM + BN) * 128, DMAS = STAGE / (1024 * WM * WN);  // bytes of a stage's images; DMAs of 1 KB a wave
+    static_assert(TN == 64 && TM % 64 == 0 && STAGE * 2 == 16384 * WM * WN && AB / 1024 % DMAS == 0, "16 KB a wave; a wave's DMAs belong to one operand");
+    extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i16 = lane & 15, q = lane >> 4;
     const int tiles = p.tiles_m * p.tiles_n;
-    const int split = blockIdx.x / tiles, tile = blockIdx.x - split * tiles;
-    const int tm = tile / p.tiles_n, tn = tile - tm * p.tiles_n;
-    const int m0 = tm * 128, n0 = tn * 128;
+    const int split = blockIdx.x / tiles, id = blockIdx.x - split * tiles;
+    int tm, tn;
+    {
+        const int x = id & 7, per = tiles >> 3, more = tiles & 7;
+        const int t = x * per + (x < more ? x : more) + (id >> 3);
+        const int band = 8 * p.tiles_n, g = t / band, in = t - g * band;               // bands of 8 tile rows, walked column by column
+        const int high = p.tiles_m - 8 * g < 8 ? p.tiles_m - 8 * g : 8;
+        tn = in / high;
+        tm = 8 * g + in - tn * high;
+    }
+    const int m0 = tm * BM, n0 = tn * BN;
     const int kb = split * p.k_per_split, ke = kb + p.k_per_split < p.K ? kb + p.k_per_split : p.K;
-    const int steps = (ke - kb + 31) / 32;
+    const int stages = (ke - kb + 63) / 64, full = (ke - kb) / 64;
     const unsigned base = (unsigned)(size_t)lds;
-    const void* zero = (const void*)g_zero_lin16;
-    asm volatile("" : "+s"(zero));
 
-    // One operand's step: 8 DMAs of 1 KB, two a wave.  KC: 16 rows x four 16-byte pieces, piece j of row r <- piece j ^ (r >> 2 & 3) (16 rows at one
-    // piece then cover all banks once); MC: four k rows x 16 pieces, piece j of row r <- j ^ 2 (r & 3 | (r >> 3 & 1) << 2).
-    // A piece outside the operand is read from a line of zeros: the sizes along k and along the rows are multiples of 8.
-    auto fetch = [&](bool mc, const u16* X, long ldx, int rows, int r0, int k0, unsigned dst) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int d = 2 * wave + e;
-            const void* src;
-            if (!mc) {
-                const int r = 16 * d + (lane >> 2), pc = (lane & 3) ^ ((r >> 2) & 3), k = k0 + 8 * pc;
-                const int row = r0 + r < rows ? r0 + r : rows - 1;
-                src = k < ke ? (const void*)(X + (long)row * ldx + k) : zero;
-            } else {
-                const int r = 4 * d + (lane >> 4), pc = (lane & 15) ^ (2 * ((r & 3) | (((r >> 3) & 1) << 2)));
-                const int k = k0 + r, c = r0 + 8 * pc;
-                src = k < ke && c < rows ? (const void*)(X + (long)k * ldx + c) : zero;
-            }
-            cdae_lds_dma16(src, dst + d * 1024);
+    // This wave's DMAs: DMAS of 1 KB, of operand A (waves of the first AB bytes) or B.  Lane l reads 16 bytes of
+    //   KC: row 8 d + l / 8, piece (l % 8) ^ f(row);     MC: k row 4 d + l / 16 of a plane, piece (l % 16) ^ 2 g(k row).
+    // Rows past the operand repeat its last row or piece: they reach results that are not written.
+    const bool isa = wave * DMAS < AB / 1024;
+    const int d0 = isa ? wave * DMAS : wave * DMAS - AB / 1024;
+    auto place = [&](bool mc, int rows, int r0, int d, int& row, int& k) {
+        if (!mc) {
+            const int r = 8 * d + (lane >> 3);
+            k = 8 * ((lane & 7) ^ (r >> 1 & 7));
+            row = r0 + r < rows ? r0 + r : rows - 1;
+        } else {
+            k = 4 * (d & 15) + (lane >> 4);
+            const int c = r0 + 128 * (d >> 4) + 8 * ((lane & 15) ^ (2 * ((k & 3) | (((k >> 3) & 1) << 2))));
+            row = c < rows ? c : (rows - 1) & ~7;
         }
     };
-    auto frag = [&](bool mc, const unsigned char* img, int r0) -> u32x4 {            // 8 k (8 q .. + 7) of row r0 + i16
-        if (!mc) {
-            const int r = r0 + i16;
-            return *reinterpret_cast<const u32x4*>(img + r * 64 + ((q ^ ((r >> 2) & 3)) * 16));
+    auto where = [&](int d, int& k) -> unsigned {                         // byte offset from the operand's stage base
+        int row;
+        if (isa) {
+            place(AMC, p.M, m0, d, row, k);
+            return (unsigned)(2 * (AMC ? k * p.lda + row : (row - m0) * p.lda + k));
         }
-        const int k = 8 * q + (i16 >> 2), pp = i16 & 3;
-        const unsigned char* src = img + k * 256 + ((((r0 >> 3) + (pp >> 1)) ^ (2 * ((k & 3) | (((k >> 3) & 1) << 2)))) * 16) + (pp & 1) * 8;
+        place(BMC, p.N, n0, d, row, k);
+        return (unsigned)(2 * (BMC ? k * p.ldb + row : (row - n0) * p.ldb + k));
+    };
+    const u16* const mine = isa ? (AMC ? p.A + (long)kb * p.lda : p.A + (long)m0 * p.lda + kb) : (BMC ? p.B + (long)kb * p.ldb : p.B + (long)n0 * p.ldb + kb);
+    const long step = isa ? (AMC ? 64 * p.lda : 64) : (BMC ? 64 * p.ldb : 64);
+    unsigned off[DMAS];
+#pragma unroll
+    for (int e = 0; e < DMAS; ++e) { int k; off[e] = where(d0 + e, k); }
+    auto fetch = [&](int s) {
+        const unsigned dst = base + (s & 1) * STAGE + wave * (DMAS * 1024);
+        const u16* src = mine + s * step;
+        if (s < full) {
+#pragma unroll
+            for (int e = 0; e < DMAS; ++e) lds_dma16_s(src, off[e], dst + e * 1024);
+        } else {                                                          // the last, partial stage: what lies past ke reads a line of zeros
+#pragma unroll 1
+            for (int e = 0; e < DMAS; ++e) {
+                int k;
+                const unsigned o = where(d0 + e, k);
+                cdae_lds_dma16(kb + 64 * s + k < ke ? (const void*)((const char*)src + o) : (const void*)g_zero_lin16, dst + e * 1024);
+            }
+        }
+    };
+
+    const int wm = wave / WN, wn = wave - wm * WN;
+    // lane offsets of the fragment reads: KC at the row's piece q (first half of a stage; the second half's is 64 bytes away, ^ 64), MC at k row 8 q + ..
+    const int kq = 8 * q + (i16 >> 2), mcs = 2 * ((kq & 3) | (((kq >> 3) & 1) << 2));
+    const int ra = (wm * TM + i16) * 128 + ((q ^ (i16 >> 1 & 7)) * 16);
+    const int rb = (wn * TN + i16) * 128 + ((q ^ (i16 >> 1 & 7)) * 16);
+    auto frag_mc = [&](const unsigned char* img, int r0, int h) -> u32x4 {      // 8 k (32 h + 8 q .. + 7) of column r0 + i16
+        const unsigned char* src = img + (r0 >> 7) * 16384 + h * 8192 + kq * 256 + (((((r0 & 127) >> 3) + ((i16 & 3) >> 1)) ^ mcs) * 16) + (i16 & 1) * 8;
         const fp16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4*)(src));
         const fp16x4 c = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4*)(src + 4 * 256));
         const u32x2 a2 = __builtin_bit_cast(u32x2, a), c2 = __builtin_bit_cast(u32x2, c);
@@ -154,44 +219,70 @@ __global__ __launch_bounds__(256, 2) void lin_tile_kernel(const LinArgs p) {
         v[0] = a2[0]; v[1] = a2[1]; v[2] = c2[0]; v[3] = c2[1];
         return v;
     };
-
-    const int wm = wave >> 1, wn = wave & 1;
-    f32x4 acc[4][4];
-#pragma unroll
-    for (int a = 0; a < 4; ++a)
-#pragma unroll
-        for (int b = 0; b < 4; ++b) acc[a][b] = (f32x4){0.f, 0.f, 0.f, 0.f};
-
-    fetch(AMC, p.A, p.lda, p.M, m0, kb, base);
-    fetch(BMC, p.B, p.ldb, p.N, n0, kb, base + OPB);
-    for (int s = 0; s < steps; ++s) {
-        const int slot = s & 1;
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        if (s + 1 < steps) {
-            fetch(AMC, p.A, p.lda, p.M, m0, kb + 32 * (s + 1), base + (slot ^ 1) * STAGE);
-            fetch(BMC, p.B, p.ldb, p.N, n0, kb + 32 * (s + 1), base + (slot ^ 1) * STAGE + OPB);
-        }
+    auto read = [&](int slot, int h, u32x4 (&fa)[FA], u32x4 (&fb)[FB]) {
         const unsigned char* as = lds + slot * STAGE;
-        const unsigned char* bs = as + OPB;
-        u32x4 fa[4], fb[4];
+        const unsigned char* bs = as + AB;
 #pragma unroll
-        for (int a = 0; a < 4; ++a) { fa[a] = frag(AMC, as, wm * 64 + a * 16); fb[a] = frag(BMC, bs, wn * 64 + a * 16); }
+        for (int b = 0; b < FB; ++b) {
+            if constexpr (BMC) fb[b] = frag_mc(bs, wn * TN + b * 16, h);
+            else fb[b] = *reinterpret_cast<const u32x4*>(bs + (rb ^ (64 * h)) + b * 2048);
+        }
+#pragma unroll
+        for (int a = 0; a < FA; ++a) {
+            if constexpr (AMC) fa[a] = frag_mc(as, wm * TM + a * 16, h);
+            else fa[a] = *reinterpret_cast<const u32x4*>(as + (ra ^ (64 * h)) + a * 2048);
+        }
+    };
+    f32x4 acc[FA][FB];
+#pragma unroll
+    for (int a = 0; a < FA; ++a)
+#pragma unroll
+        for (int b = 0; b < FB; ++b) acc[a][b] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    auto multiply = [&](u32x4 (&fa)[FA], u32x4 (&fb)[FB]) {
+#pragma unroll
+        for (int a = 0; a < FA; ++a)
+#pragma unroll
+            for (int b = 0; b < FB; ++b) acc[a][b] = Mfma<T>::go(fb[b], fa[a], acc[a][b]);       // rows of the result: n (4 q + r), columns: m (i16)
+    };
+
+    u32x4 fa[2][FA], fb[2][FB];
+    fetch(0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (stages > 1) fetch(1);
+    read(0, 0, fa[0], fb[0]);
+    for (int s = 0; s < stages; ++s) {
+        read(s & 1, 1, fa[1], fb[1]);
+        multiply(fa[0], fb[0]);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                  // stage s + 1 has landed (here; behind the barrier for every wave) ...
+        __syncthreads();                                                  // ... and every wave has read the whole of stage s
+        if (s + 2 < stages) fetch(s + 2);
+        if (s + 1 < stages) read((s + 1) & 1, 0, fa[0], fb[0]);
+        multiply(fa[1], fb[1]);
+    }
+
+    // Epilogue through the wave's own 16 KB of the stages, 64 rows at a time, so that one short loop serves every variant (unrolled over the accumulators
+    // it was 60 000 instructions) and rows leave as whole lines.  Row r's 16-byte piece j (4 columns) lies at j ^ (r & 15).
+    unsigned char* const own = lds + wave * 16384;
+    const int cl = 8 * (lane & 7), n = n0 + wn * TN + cl, have = p.N - n;
+    float bias[8];
+    load_bias<T, 8>(p, n, have, bias);
+#pragma unroll
+    for (int h = 0; h < FA / 4; ++h) {
 #pragma unroll
         for (int a = 0; a < 4; ++a)
 #pragma unroll
-            for (int b = 0; b < 4; ++b) acc[a][b] = Mfma<T>::go(fb[b], fa[a], acc[a][b]);       // rows of the result: n (4 q + r), columns: m (i16)
-    }
-#pragma unroll
-    for (int a = 0; a < 4; ++a) {
-        const int m = m0 + wm * 64 + a * 16 + i16;
-        if (m >= p.M) continue;
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const int n = n0 + wn * 64 + b * 16 + 4 * q;
-            float v[4] = {acc[a][b][0], acc[a][b][1], acc[a][b][2], acc[a][b][3]};
-            if (p.splits > 1) { if (n < p.N) stv_n<float, 4>(p.slab + ((long)split * p.M + m) * p.N + n, p.N - n, v); }
-            else finish_row<T, 4>(p, m, n, p.N - n, v);
+            for (int b = 0; b < FB; ++b) *reinterpret_cast<f32x4*>(own + (16 * a + i16) * 256 + (((4 * b + q) ^ i16) * 16)) = acc[4 * h + a][b];
+#pragma unroll 1
+        for (int i = 0; i < 8; ++i) {
+            const int r = 8 * i + (lane >> 3), m = m0 + wm * TM + 64 * h + r;
+            const f32x4 lo = *reinterpret_cast<const f32x4*>(own + r * 256 + ((((cl >> 2)) ^ (r & 15)) * 16));
+            const f32x4 hi = *reinterpret_cast<const f32x4*>(own + r * 256 + ((((cl >> 2) + 1) ^ (r & 15)) * 16));
+            float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            if (m < p.M && have > 0) {
+                if (p.splits > 1) stv_n<float, 8>(p.slab + ((long)split * p.M + m) * p.N + n, have, v);
+                else finish_row<T, 8>(p, m, n, have, v, bias);
+            }
         }
     }
 }
@@ -210,7 +301,9 @@ __global__ __launch_bounds__(256) void lin_finish_kernel(const LinArgs p) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] += t[e];
         }
-        finish_row<T, 8>(p, m, n, have, v);
+        float bias[8];
+        load_bias<T, 8>(p, n, have, bias);
+        finish_row<T, 8>(p, m, n, have, v, bias);
     }
 }
 
@@ -289,16 +382,19 @@ long up8(long v) { return (v + 7) / 8 * 8; }
 bool al16(const void* p) { return ((size_t)p & 15) == 0; }
 size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 
-// splits of the sum over k: where the tiles alone leave most of the 512 block slots (two a CU) empty, and a split keeps at least 256 of k
-int splits_of(int M, int N, int K) {
-    const long tiles = (long)((M + 127) / 128) * ((N + 127) / 128);
+// Tile and splits of the sum over k.  256 x 256 tiles (one block a CU) where they alone fill the CUs; else 128 x 128 tiles (two a CU), and where those
+// leave most of the 512 slots empty the sum is split, a split keeping at least 256 of k.
+struct Plan { int bm, splits; };
+Plan plan(int M, int N, int K) {
+    const long big = ((M + 255L) / 256) * ((N + 255L) / 256), tiles = ((M + 127L) / 128) * ((N + 127L) / 128);
+    if (big >= 256) return {256, 1};
     long s = 512 / (tiles > 0 ? tiles : 1);
     if (s > K / 256) s = K / 256;
     if (s > 64) s = 64;
-    return s < 1 ? 1 : (int)s;
+    return {128, s < 1 ? 1 : (int)s};
 }
 size_t gemm_ws(int M, int N, int K) {
-    const int s = splits_of(M, N, K);
+    const int s = plan(M, N, K).splits;
     return s > 1 ? up256((size_t)s * M * N * 4) : 0;
 }
 
@@ -315,18 +411,27 @@ int prepare(const u16*& X, long& ldx, long rows, int cols, char*& ws, hipStream_
     return hipGetLastError() == hipSuccess ? 0 : cdae_fail("lin16: launch failed");
 }
 
+template <class T, bool AMC, bool BMC, int BM, int WN>
+int launch_tiles(const LinArgs& p, unsigned blocks, hipStream_t st) {
+    constexpr int smem = 2 * 2 * BM * 128;
+    auto* kernel = &lin_tile_kernel<T, AMC, BMC, BM, BM, 2, WN>;
+    if (smem > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, smem) != hipSuccess)
+        return cdae_fail("lin16: hipFuncSetAttribute(max dynamic LDS) failed");
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(128 * WN), smem, st, p);
+    return hipGetLastError() == hipSuccess ? 0 : cdae_fail("lin16: launch failed");
+}
 template <class T, bool AMC, bool BMC>
 int product(LinArgs p, char* ws, hipStream_t st) {
-    p.tiles_m = (p.M + 127) / 128; p.tiles_n = (p.N + 127) / 128;
-    // (rows of an MC operand are padded to 8 values, so the kernel may see up to 7 columns more than there are: it reads them, and writes none)
-    p.splits = splits_of(p.M, p.N, p.K);
-    p.k_per_split = ((p.K + p.splits - 1) / p.splits + 31) / 32 * 32;
+    const Plan pl = plan(p.M, p.N, p.K);
+    p.tiles_m = (p.M + pl.bm - 1) / pl.bm; p.tiles_n = (p.N + pl.bm - 1) / pl.bm;
+    p.splits = pl.splits;
+    p.k_per_split = ((p.K + p.splits - 1) / p.splits + 63) / 64 * 64;
     p.splits = (p.K + p.k_per_split - 1) / p.k_per_split;
     p.slab = (float*)ws;
     const long blocks = (long)p.tiles_m * p.tiles_n * p.splits;
-    if (blocks > (1L << 23)) return cdae_fail("lin16: product too large");
-    hipLaunchKernelGGL((lin_tile_kernel<T, AMC, BMC>), dim3((unsigned)blocks), dim3(256), 0, st, p);
-    if (hipGetLastError() != hipSuccess) return cdae_fail("lin16: launch failed");
+    // (a lane's offset inside a stage is 32 bits: 256 rows, or 64 k rows and the columns)
+    if (blocks > (1L << 22) || 512 * (AMC ? p.lda / 4 + p.M / 256 : p.lda) >= (1L << 32) || 512 * (BMC ? p.ldb / 4 + p.N / 256 : p.ldb) >= (1L << 32)) return cdae_fail("lin16: product too large");
+    if (pl.bm == 256 ? launch_tiles<T, AMC, BMC, 256, 4>(p, (unsigned)blocks, st) : launch_tiles<T, AMC, BMC, 128, 2>(p, (unsigned)blocks, st)) return -1;
     if (p.splits > 1) {
         const long g = ((long)p.M * ((p.N + 7) / 8) + 255) / 256;
         hipLaunchKernelGGL((lin_finish_kernel<T>), dim3((unsigned)(g < 8192 ? g : 8192)), dim3(256), 0, st, p);

@@ -8,6 +8,8 @@
 #include <hip/hip_runtime.h>
 #include <math.h>
 
+#include <type_traits>
+
 #include "cdae.h"
 #include "block_common.h"
 #include "cdae_internal.h"
@@ -41,30 +43,36 @@ __device__ __forceinline__ float normal_cdf(float z, float& e) {
 }
 __device__ __forceinline__ float gelu_tanh_arg(float z) { return 1.5957691216057308f * z * fmaf(0.044715f * z, z, 1.f); }      // 0.5 (1 + tanh a) = logistic(2 a)
 
-__device__ __forceinline__ float act_fwd(float z, int act) {
-    switch (act) {
-        case L_SILU: return z * logistic(z);
-        case L_RELU: return z > 0.f ? z : (z != z ? z : 0.f);
-        case L_GELU: { float e; return z * normal_cdf(z, e); }
-        case L_GELU_TANH: return z * logistic(gelu_tanh_arg(z));
-        default: return z;
-    }
+template <int ACT>
+__device__ __forceinline__ float act_of(float z) {
+    if constexpr (ACT == L_SILU) return z * logistic(z);
+    else if constexpr (ACT == L_RELU) return z < 0.f ? 0.f : z;
+    else if constexpr (ACT == L_GELU) { float e; return z * normal_cdf(z, e); }
+    else if constexpr (ACT == L_GELU_TANH) return z * logistic(gelu_tanh_arg(z));
+    else return z;
 }
-__device__ __forceinline__ float act_slope(float z, int act) {
-    switch (act) {
-        case L_SILU: { const float s = logistic(z); return s * fmaf(z, 1.f - s, 1.f); }
-        case L_RELU: return z > 0.f ? 1.f : (z != z ? z : 0.f);
-        case L_GELU: { float e; const float c = normal_cdf(z, e); return fmaf(0.3989422804014327f * z, e, c); }
-        case L_GELU_TANH: {
-            const float s = logistic(gelu_tanh_arg(z));
-            return s * fmaf(z * (1.f - s), 1.5957691216057308f * fmaf(0.134145f * z, z, 1.f), 1.f);
-        }
-        default: return 1.f;
-    }
+template <int ACT>
+__device__ __forceinline__ float slope_of(float z) {
+    if constexpr (ACT == L_SILU) { const float s = logistic(z); return s * fmaf(z, 1.f - s, 1.f); }
+    else if constexpr (ACT == L_RELU) return z > 0.f ? 1.f : z * 0.f;                 // (not a number stays one)
+    else if constexpr (ACT == L_GELU) { float e; const float c = normal_cdf(z, e); return fmaf(0.3989422804014327f * z, e, c); }
+    else if constexpr (ACT == L_GELU_TANH) {
+        const float s = logistic(gelu_tanh_arg(z));
+        return s * fmaf(z * (1.f - s), 1.5957691216057308f * fmaf(0.134145f * z, z, 1.f), 1.f);
+    } else return 1.f;
 }
+// CALL(activation) with the number as a constant: one branch for all values of a thread
+#define LIN_ACT(act, CALL)                                            \
+    switch (act) {                                                    \
+        case L_SILU: CALL(L_SILU); break;                             \
+        case L_RELU: CALL(L_RELU); break;                             \
+        case L_GELU: CALL(L_GELU); break;                             \
+        case L_GELU_TANH: CALL(L_GELU_TANH); break;                   \
+        default: break;                                               \
+    }
 // The pre-activation is kept for the backward in f16 whatever the rows' type: its 11 bits cost the slope a quarter of what the rounding of dz to
-// bf16 costs, and where f16 ends (65504) every slope has long reached its limit, so larger values are clamped there.
-__device__ __forceinline__ _Float16 keep_z(float z) { return (_Float16)(fabsf(z) > 65504.f ? copysignf(65504.f, z) : z); }
+// bf16 costs.  Beyond f16's range it becomes infinite, and the slope there is taken at the range's end, where every slope has long reached its limit.
+__device__ __forceinline__ float kept_z(F16 v) { const float z = ld1(v); return fabsf(z) > 65504.f ? copysignf(65504.f, z) : z; }
 
 struct LinArgs {
     const u16* A; long lda;                 // KC: [M][K], MC: [K][M]
@@ -87,9 +95,9 @@ template <> struct Mfma<F16> {
     }
 };
 
-// v[0..n) of row m from column n0: bias, activation, residual, rounding
+// v[0..n) of row m from column n0: bias, activation, residual (in r), rounding
 template <class T, int V>
-__device__ __forceinline__ void finish_row(const LinArgs& p, long m, int n0, int n, float (&v)[V], const float (&bias)[V]) {
+__device__ __forceinline__ void finish_row(const LinArgs& p, long m, int n0, int n, float (&v)[V], const float (&bias)[V], const Pack<T, V>& r) {
     if (n <= 0) return;
 #pragma unroll
     for (int i = 0; i < V; ++i) v[i] += bias[i];
@@ -97,22 +105,28 @@ __device__ __forceinline__ void finish_row(const LinArgs& p, long m, int n0, int
         _Float16* zp = p.z + m * p.ldz + n0;
         Pack<F16, V> k;
 #pragma unroll
-        for (int i = 0; i < V; ++i) k.v[i].h = keep_z(v[i]);
+        for (int i = 0; i < V; ++i) k.v[i].h = (_Float16)v[i];
         if (n >= V) *reinterpret_cast<Pack<F16, V>*>(zp) = k;
         else
 #pragma unroll
             for (int i = 0; i < V; ++i) if (i < n) zp[i] = k.v[i].h;
     }
-    if (p.act != L_NONE)
+#define LIN_CALL(A) _Pragma("unroll") for (int i = 0; i < V; ++i) v[i] = act_of<A>(v[i])
+    LIN_ACT(p.act, LIN_CALL)
+#undef LIN_CALL
+    if (p.res)
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = act_fwd(v[i], p.act);
-    if (p.res) {
-        float t[V];
-        ldv_n<T, V>(reinterpret_cast<const T*>(p.res) + m * p.ldres + n0, n, t);
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[i] += t[i];
-    }
+        for (int i = 0; i < V; ++i) v[i] += ld1(r.v[i]);
     stv_n<T, V>(reinterpret_cast<T*>(p.y) + m * p.ldy + n0, n, v);
+}
+// the residual of a row's n values (present ones only)
+template <class T, int V>
+__device__ __forceinline__ void load_res(const LinArgs& p, long m, int n0, int n, Pack<T, V>& r) {
+    const T* at = reinterpret_cast<const T*>(p.res) + m * p.ldres + n0;
+    if (n >= V) r = *reinterpret_cast<const Pack<T, V>*>(at);
+    else
+#pragma unroll
+        for (int i = 0; i < V; ++i) if (i < n) r.v[i] = at[i];
 }
 template <class T, int V>
 __device__ __forceinline__ void load_bias(const LinArgs& p, int n0, int n, float (&b)[V]) {
@@ -127,19 +141,21 @@ __device__ __forceinline__ void lds_dma16_s(const void* base, unsigned off, unsi
 }
 
 // One BM x BN tile of the result (and one range of k): WM x WN waves, 64 k a stage.
-//   * stages arrive by LDS-DMA in two slots; the request for stage S + 2 goes out when the second half of stage S begins, one barrier a stage;
-//   * the fragments of the next 32 k are read from LDS while these 32 k run on the matrix cores (two register sets), so no product waits for LDS;
-//   * operand images: KC, rows of 128 bytes (whole cache lines: with 64-byte rows each line was fetched twice, 581 us for 16384 x 8192 x 2048 where
-//     the MC x MC product of the same size took 458) whose 16-byte piece j lies at j ^ f(row); MC, 128-column planes of 256-byte k rows whose piece j lies
-//     at j ^ 2 g(k row), read through the transpose read.  f, g spread the rows that one read touches over all banks; the permutation is applied to
-//     the global address of the DMA lane;
+//   * stages arrive by LDS-DMA in SLOTS slots; the request for stage S + SLOTS goes out when the second half of stage S begins; counted vmcnt, one
+//     barrier a stage;
+//   * the fragments of the next 32 k are read from LDS while these 32 k run on the matrix cores (two register sets); reads, requests and products
+//     are interleaved by hand;
+//   * operand images: KC, rows of 128 bytes (whole cache lines: with 64-byte rows each line was fetched twice, 581 us for that product) whose
+//     16-byte piece j lies at j ^ f(row); MC, planes of up to 128 columns whose k row's piece j lies at j ^ 2 g(k row), read through the transpose
+//     read.  f, g spread the rows that one read touches over all banks; the permutation is applied to the global address of the DMA lane;
 //   * the operands are swapped in the instruction (B in the A slot): a lane's four accumulators are four consecutive columns of one row;
 //   * blocks that run on one XCD (block number mod 8) take neighbouring tiles, 8 rows of tiles at a time: an operand's panel is read from HBM once an XCD.
-template <class T, bool AMC, bool BMC, int BM, int BN, int WM, int WN>
+template <class T, bool AMC, bool BMC, int BM, int BN, int WM, int WN, int SLOTS>
 __global__ __launch_bounds__(64 * WM * WN, 2) void lin_tile_kernel(const LinArgs p) {
     constexpr int TM = BM / WM, TN = BN / WN, FA = TM / 16, FB = TN / 16;                 // a wave's part and its fragments
     constexpr int AB = BM * 128, STAGE = (BM + BN) * 128, DMAS = STAGE / (1024 * WM * WN);  // bytes of a stage's images; DMAs of 1 KB a wave
-    static_assert(TN == 64 && TM % 64 == 0 && STAGE * 2 == 16384 * WM * WN && AB / 1024 % DMAS == 0, "16 KB a wave; a wave's DMAs belong to one operand");
+    constexpr int PA = BM < 128 ? BM : 128, PB = BN < 128 ? BN : 128;                     // columns of an MC plane
+    static_assert(TN == 64 && AB / 1024 % DMAS == 0 && PA == PB, "64 columns a wave; a wave's DMAs belong to one operand");
     extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i16 = lane & 15, q = lane >> 4;
@@ -160,7 +176,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void lin_tile_kernel(const LinArgs
     const unsigned base = (unsigned)(size_t)lds;
 
     // This wave's DMAs: DMAS of 1 KB, of operand A (waves of the first AB bytes) or B.  Lane l reads 16 bytes of
-    //   KC: row 8 d + l / 8, piece (l % 8) ^ f(row);     MC: k row 4 d + l / 16 of a plane, piece (l % 16) ^ 2 g(k row).
+    //   KC: row 8 d + l / 8, piece (l % 8) ^ f(row);     MC (128 columns): k row 4 d + l / 16 of a plane, piece (l % 16) ^ 2 g(k row);
+    //   MC (64 columns): k row 8 d + l / 8, piece (l % 8) ^ 2 g(k row).
     // Rows past the operand repeat its last row or piece: they reach results that are not written.
     const bool isa = wave * DMAS < AB / 1024;
     const int d0 = isa ? wave * DMAS : wave * DMAS - AB / 1024;
@@ -170,8 +187,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void lin_tile_kernel(const LinArgs
             k = 8 * ((lane & 7) ^ (r >> 1 & 7));
             row = r0 + r < rows ? r0 + r : rows - 1;
         } else {
-            k = 4 * (d & 15) + (lane >> 4);
-            const int c = r0 + 128 * (d >> 4) + 8 * ((lane & 15) ^ (2 * ((k & 3) | (((k >> 3) & 1) << 2))));
+            k = PA == 128 ? 4 * (d & 15) + (lane >> 4) : 8 * d + (lane >> 3);
+            const int c = PA == 128 ? r0 + 128 * (d >> 4) + 8 * ((lane & 15) ^ (2 * ((k & 3) | (((k >> 3) & 1) << 2)))) : r0 + 8 * ((lane & 7) ^ (2 * ((k >> 1 & 1) | (k >> 3 & 1) << 1)));
             row = c < rows ? c : (rows - 1) & ~7;
         }
     };
@@ -190,7 +207,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void lin_tile_kernel(const LinArgs
 #pragma unroll
     for (int e = 0; e < DMAS; ++e) { int k; off[e] = where(d0 + e, k); }
     auto fetch = [&](int s) {
-        const unsigned dst = base + (s & 1) * STAGE + wave * (DMAS * 1024);
+        const unsigned dst = base + s % SLOTS * STAGE + wave * (DMAS * 1024);
         const u16* src = mine + s * step;
         if (s < full) {
 #pragma unroll
@@ -207,103 +224,148 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void lin_tile_kernel(const LinArgs
 
     const int wm = wave / WN, wn = wave - wm * WN;
     // lane offsets of the fragment reads: KC at the row's piece q (first half of a stage; the second half's is 64 bytes away, ^ 64), MC at k row 8 q + ..
-    const int kq = 8 * q + (i16 >> 2), mcs = 2 * ((kq & 3) | (((kq >> 3) & 1) << 2));
+    const int kq = 8 * q + (i16 >> 2), mcs = PA == 128 ? 2 * ((kq & 3) | (((kq >> 3) & 1) << 2)) : 2 * ((kq >> 1 & 1) | (kq >> 3 & 1) << 1);
     const int ra = (wm * TM + i16) * 128 + ((q ^ (i16 >> 1 & 7)) * 16);
     const int rb = (wn * TN + i16) * 128 + ((q ^ (i16 >> 1 & 7)) * 16);
     auto frag_mc = [&](const unsigned char* img, int r0, int h) -> u32x4 {      // 8 k (32 h + 8 q .. + 7) of column r0 + i16
-        const unsigned char* src = img + (r0 >> 7) * 16384 + h * 8192 + kq * 256 + (((((r0 & 127) >> 3) + ((i16 & 3) >> 1)) ^ mcs) * 16) + (i16 & 1) * 8;
+        const unsigned char* src = img + r0 / PA * (PA * 128) + h * (PA * 64) + kq * (PA * 2) + ((((r0 % PA >> 3) + ((i16 & 3) >> 1)) ^ mcs) * 16) + (i16 & 1) * 8;
         const fp16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4*)(src));
-        const fp16x4 c = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4*)(src + 4 * 256));
+        const fp16x4 c = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4*)(src + 8 * PA));
         const u32x2 a2 = __builtin_bit_cast(u32x2, a), c2 = __builtin_bit_cast(u32x2, c);
         u32x4 v;
         v[0] = a2[0]; v[1] = a2[1]; v[2] = c2[0]; v[3] = c2[1];
         return v;
     };
-    auto read = [&](int slot, int h, u32x4 (&fa)[FA], u32x4 (&fb)[FB]) {
+    auto read_a = [&](int slot, int h, int a) -> u32x4 {
         const unsigned char* as = lds + slot * STAGE;
-        const unsigned char* bs = as + AB;
-#pragma unroll
-        for (int b = 0; b < FB; ++b) {
-            if constexpr (BMC) fb[b] = frag_mc(bs, wn * TN + b * 16, h);
-            else fb[b] = *reinterpret_cast<const u32x4*>(bs + (rb ^ (64 * h)) + b * 2048);
-        }
-#pragma unroll
-        for (int a = 0; a < FA; ++a) {
-            if constexpr (AMC) fa[a] = frag_mc(as, wm * TM + a * 16, h);
-            else fa[a] = *reinterpret_cast<const u32x4*>(as + (ra ^ (64 * h)) + a * 2048);
-        }
+        if constexpr (AMC) return frag_mc(as, wm * TM + a * 16, h);
+        else return *reinterpret_cast<const u32x4*>(as + (ra ^ (64 * h)) + a * 2048);
+    };
+    auto read_b = [&](int slot, int h, int b) -> u32x4 {
+        const unsigned char* bs = lds + slot * STAGE + AB;
+        if constexpr (BMC) return frag_mc(bs, wn * TN + b * 16, h);
+        else return *reinterpret_cast<const u32x4*>(bs + (rb ^ (64 * h)) + b * 2048);
     };
     f32x4 acc[FA][FB];
 #pragma unroll
     for (int a = 0; a < FA; ++a)
 #pragma unroll
         for (int b = 0; b < FB; ++b) acc[a][b] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    auto multiply = [&](u32x4 (&fa)[FA], u32x4 (&fb)[FB]) {
-#pragma unroll
-        for (int a = 0; a < FA; ++a)
-#pragma unroll
-            for (int b = 0; b < FB; ++b) acc[a][b] = Mfma<T>::go(fb[b], fa[a], acc[a][b]);       // rows of the result: n (4 q + r), columns: m (i16)
-    };
-
+    // 32 k on the matrix cores from set `cur`, a row of fragments at a time; between the rows the next half's fragments are read into the other set
+    // and (FETCH) the DMAs of a later stage issued.  All of a stage's DMAs in one go behind the barrier held every wave up for the 16 cycles a
+    // KB that the four or eight waves' requests take: 1665 cycles a stage of a lone 128 x 128 block against 512 of products.
     u32x4 fa[2][FA], fb[2][FB];
-    fetch(0);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    auto half = [&](auto fetching, int cur, bool more, int slot, int h, const u16* src, unsigned dst) {
+        constexpr bool FETCH = decltype(fetching)::value;
+#pragma unroll
+        for (int a = 0; a < FA; ++a) {
+            if constexpr (FETCH)
+#pragma unroll
+                for (int e = a * DMAS / FA; e < (a + 1) * DMAS / FA; ++e) lds_dma16_s(src, off[e], dst + e * 1024);
+            if (more) {
+#pragma unroll
+                for (int b = a * FB / FA; b < (a + 1) * FB / FA; ++b) fb[cur ^ 1][b] = read_b(slot, h, b);
+                fa[cur ^ 1][a] = read_a(slot, h, a);
+            }
+#pragma unroll
+            for (int b = 0; b < FB; ++b) acc[a][b] = Mfma<T>::go(fb[cur][b], fa[cur][a], acc[a][b]);       // rows of the result: n (4 q + r), columns: m (i16)
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    using Yes = std::true_type;
+    using No = std::false_type;
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s) if (s < stages) fetch(s);
+    if (stages >= SLOTS) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((SLOTS - 1) * DMAS) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (stages > 1) fetch(1);
-    read(0, 0, fa[0], fb[0]);
-    for (int s = 0; s < stages; ++s) {
-        read(s & 1, 1, fa[1], fb[1]);
-        multiply(fa[0], fb[0]);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                  // stage s + 1 has landed (here; behind the barrier for every wave) ...
-        __syncthreads();                                                  // ... and every wave has read the whole of stage s
-        if (s + 2 < stages) fetch(s + 2);
-        if (s + 1 < stages) read((s + 1) & 1, 0, fa[0], fb[0]);
-        multiply(fa[1], fb[1]);
+#pragma unroll
+    for (int b = 0; b < FB; ++b) fb[0][b] = read_b(0, 0, b);
+#pragma unroll
+    for (int a = 0; a < FA; ++a) fa[0][a] = read_a(0, 0, a);
+    int slot = 0, s = 0;
+    // behind the barrier: stage s + 1 has landed for every wave, and every wave has read the whole of stage s, whose slot is then free
+    for (; s + SLOTS < full; ++s) {
+        const int after = slot == SLOTS - 1 ? 0 : slot + 1;
+        half(No{}, 0, true, slot, 1, nullptr, 0u);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((SLOTS - 2) * DMAS) : "memory");
+        __syncthreads();
+        half(Yes{}, 1, true, after, 0, mine + (s + SLOTS) * step, base + slot * STAGE + wave * (DMAS * 1024));
+        slot = after;
+    }
+    for (; s < stages; ++s) {                                             // the last stages: nothing or a partial stage left to request
+        const int after = slot == SLOTS - 1 ? 0 : slot + 1;
+        half(No{}, 0, true, slot, 1, nullptr, 0u);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (s + SLOTS < stages) fetch(s + SLOTS);
+        half(No{}, 1, s + 1 < stages, after, 0, nullptr, 0u);
+        slot = after;
     }
 
-    // Epilogue through the wave's own 16 KB of the stages, 64 rows at a time, so that one short loop serves every variant (unrolled over the accumulators
-    // it was 60 000 instructions) and rows leave as whole lines.  Row r's 16-byte piece j (4 columns) lies at j ^ (r & 15).
-    unsigned char* const own = lds + wave * 16384;
+    // Epilogue through the wave's own part of the stages, up to 64 rows at a time, so that one short loop serves every variant (unrolled over the
+    // accumulators it was 60 000 instructions) and rows leave as whole lines.  Row r's 16-byte piece j (4 columns) lies at j ^ (r & 15).
+    constexpr int PR = FA < 4 ? FA : 4, RB = 2 * PR < 4 ? 2 * PR : 4;     // 16-row groups of a pass; 8-row groups whose residuals are on their way together
+    static_assert(PR * 4096 * WM * WN <= SLOTS * STAGE, "the epilogue fits the stages");
+    unsigned char* const own = lds + wave * (PR * 4096);
     const int cl = 8 * (lane & 7), n = n0 + wn * TN + cl, have = p.N - n;
     float bias[8];
     load_bias<T, 8>(p, n, have, bias);
 #pragma unroll
-    for (int h = 0; h < FA / 4; ++h) {
+    for (int h = 0; h < FA / PR; ++h) {
 #pragma unroll
-        for (int a = 0; a < 4; ++a)
+        for (int a = 0; a < PR; ++a)
 #pragma unroll
-            for (int b = 0; b < FB; ++b) *reinterpret_cast<f32x4*>(own + (16 * a + i16) * 256 + (((4 * b + q) ^ i16) * 16)) = acc[4 * h + a][b];
+            for (int b = 0; b < FB; ++b) *reinterpret_cast<f32x4*>(own + (16 * a + i16) * 256 + (((4 * b + q) ^ i16) * 16)) = acc[PR * h + a][b];
 #pragma unroll 1
-        for (int i = 0; i < 8; ++i) {
-            const int r = 8 * i + (lane >> 3), m = m0 + wm * TM + 64 * h + r;
-            const f32x4 lo = *reinterpret_cast<const f32x4*>(own + r * 256 + ((((cl >> 2)) ^ (r & 15)) * 16));
-            const f32x4 hi = *reinterpret_cast<const f32x4*>(own + r * 256 + ((((cl >> 2) + 1) ^ (r & 15)) * 16));
-            float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-            if (m < p.M && have > 0) {
-                if (p.splits > 1) stv_n<float, 8>(p.slab + ((long)split * p.M + m) * p.N + n, have, v);
-                else finish_row<T, 8>(p, m, n, have, v, bias);
+        for (int i = 0; i < 2 * PR; i += RB) {
+            const int r0 = 8 * i + (lane >> 3);
+            const long mr = m0 + wm * TM + 16 * PR * h + r0;
+            Pack<T, 8> res[RB];
+            if (p.res && p.splits == 1)
+#pragma unroll
+                for (int e = 0; e < RB; ++e) load_res<T, 8>(p, mr + 8 * e < p.M ? mr + 8 * e : p.M - 1, have > 0 ? n : 0, have > 0 ? have : 0, res[e]);
+#pragma unroll
+            for (int e = 0; e < RB; ++e) {
+                const int r = r0 + 8 * e;
+                const long m = mr + 8 * e;
+                const f32x4 lo = *reinterpret_cast<const f32x4*>(own + r * 256 + (((cl >> 2) ^ (r & 15)) * 16));
+                const f32x4 hi = *reinterpret_cast<const f32x4*>(own + r * 256 + ((((cl >> 2) + 1) ^ (r & 15)) * 16));
+                float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                if (m < p.M && have > 0) {
+                    if (p.splits > 1) stv_n<float, 8>(p.slab + ((long)split * p.M + m) * p.N + n, have, v);
+                    else finish_row<T, 8>(p, m, n, have, v, bias, res[e]);
+                }
             }
         }
     }
 }
 
-// partial sums of the splits, added in order, then the epilogue: 8 columns a thread
+// partial sums of the splits, added in order, then the epilogue: 4 columns a thread, eight splits in flight
 template <class T>
 __global__ __launch_bounds__(256) void lin_finish_kernel(const LinArgs p) {
-    const long per = (p.N + 7) / 8, total = per * p.M;
+    const long per = (p.N + 3) / 4, total = per * p.M, plane = (long)p.M * p.N;
     for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
         const long m = i / per;
-        const int n = (int)(i - m * per) * 8, have = p.N - n;
-        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        for (int s = 0; s < p.splits; ++s) {
-            float t[8];
-            ldv_n<float, 8>(p.slab + ((long)s * p.M + m) * p.N + n, have, t);
+        const int n = (int)(i - m * per) * 4, have = p.N - n;
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        const float* at = p.slab + m * p.N + n;
+        if (have >= 4) {
+#pragma unroll 8
+            for (int s = 0; s < p.splits; ++s) {
+                const Pack<float, 4> t = *reinterpret_cast<const Pack<float, 4>*>(at + s * plane);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += t[e];
+                for (int e = 0; e < 4; ++e) v[e] += t.v[e];
+            }
+        } else {
+            for (int s = 0; s < p.splits; ++s)
+                for (int e = 0; e < have; ++e) v[e] += at[s * plane + e];
         }
-        float bias[8];
-        load_bias<T, 8>(p, n, have, bias);
-        finish_row<T, 8>(p, m, n, have, v, bias);
+        float bias[4];
+        load_bias<T, 4>(p, n, have, bias);
+        Pack<T, 4> res;
+        if (p.res) load_res<T, 4>(p, m, n, have, res);
+        finish_row<T, 4>(p, m, n, have, v, bias, res);
     }
 }
 
@@ -326,37 +388,65 @@ __global__ __launch_bounds__(256) void lin_pad_kernel(const u16* __restrict__ sr
     }
 }
 
-// dz = dy o act'(z) (written where wanted) and its column sums over a block's rows.  A block: 256 columns x 8 row lanes, 8 columns a thread.
-template <class T>
-__global__ __launch_bounds__(256) void lin_slope_kernel(const T* __restrict__ dy, long lddy, const _Float16* __restrict__ z, long ldz, T* __restrict__ dz, long lddz,
+// dz = dy o act'(z) (written where wanted) and its column sums over a block's rows.  An HBM stream (three values of 2 bytes a result).  A block: 256
+// columns x 8 lanes of rows, 8 columns a thread, four rows in flight.  Loads and stores have no branches around them: the last thread of a row takes
+// the row's LAST 8 values (its neighbour's are among them, written twice with the same value and summed once), rows past the block's end repeat its last.
+// SMALL: rows of fewer than 8 values.
+template <class T, bool SMALL>
+__global__ __launch_bounds__(256) void lin_slope_kernel(const T* __restrict__ dy, long lddy, const F16* __restrict__ z, long ldz, T* __restrict__ dz, long lddz,
                                                         float* __restrict__ part, int M, int N, int rows_per_block, int ncb, int act) {
+    constexpr int U = 4;
     __shared__ float sh[8][256];
     const int cb = blockIdx.x % ncb, rb = blockIdx.x / ncb;
     const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
-    const int c = cb * 256 + cl * 8, have = N - c;
+    const int want = cb * 256 + cl * 8, c = SMALL ? 0 : want < N - 8 ? want : N - 8;
     const long r0 = (long)rb * rows_per_block, r1 = r0 + rows_per_block < M ? r0 + rows_per_block : M;
     float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (have > 0)
-        for (long r = r0 + rl; r < r1; r += 8) {
-            float g[8];
-            ldv_n<T, 8>(dy + r * lddy + c, have, g);
-            if (act != L_NONE) {
-                float zz[8];
-                ldv_n<F16, 8>(reinterpret_cast<const F16*>(z) + r * ldz + c, have, zz);
+    for (long r = r0 + rl; r < r1; r += 8 * U) {
+        Pack<T, 8> g[U];
+        Pack<F16, 8> k[U];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) g[e] *= act_slope(zz[e], act);
-            }
-            if (dz) {
-                if (have >= 8 || c + 8 <= lddz) {                         // (a padded row takes its zeros along)
-                    stv<T, 8>(dz + r * lddz + c, g);
-                } else stv_n<T, 8>(dz + r * lddz + c, have, g);
-            }
+        for (int u = 0; u < U; ++u) {
+            const long rr = r + 8 * u < r1 ? r + 8 * u : r1 - 1;
+            if constexpr (SMALL) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s[e] += g[e];
+                for (int e = 0; e < 8; ++e) { g[u].v[e] = dy[rr * lddy + (e < N ? e : N - 1)]; if (act != L_NONE) k[u].v[e] = z[rr * ldz + (e < N ? e : N - 1)]; }
+            } else {
+                g[u] = *reinterpret_cast<const Pack<T, 8>*>(dy + rr * lddy + c);
+                if (act != L_NONE) k[u] = *reinterpret_cast<const Pack<F16, 8>*>(z + rr * ldz + c);
+            }
         }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const bool live = r + 8 * u < r1;
+            const long rr = live ? r + 8 * u : r1 - 1;
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = ld1(g[u].v[e]);
+#define LIN_CALL(A) _Pragma("unroll") for (int e = 0; e < 8; ++e) v[e] *= slope_of<A>(kept_z(k[u].v[e]))
+            LIN_ACT(act, LIN_CALL)
+#undef LIN_CALL
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[e] += live ? v[e] : 0.f;
+            if (dz) {
+                if constexpr (SMALL) {
+                    if (cl == 0)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) st1(dz[rr * lddz + e], e < N ? v[e] : 0.f);
+                } else {
+                    stv<T, 8>(dz + rr * lddz + c, v);
+                    if (N & 7 && want <= N && want + 8 > N)                // the row's padding to a multiple of 8
+                        for (int e = N; e < lddz; ++e) st1(dz[rr * lddz + e], 0.f);
+                }
+            }
+        }
+    }
     if (!part) return;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sh[rl][cl * 8 + e] = s[e];
+    for (int e = 0; e < 8; ++e) {
+        const int at = c + e - cb * 256;                                   // (columns before this thread's own are its neighbour's sums too)
+        if (SMALL ? cl == 0 : c + e >= want) sh[rl][at] = s[e];
+    }
     __syncthreads();
     const int cc = cb * 256 + threadIdx.x;
     if (cc < N) {
@@ -366,32 +456,40 @@ __global__ __launch_bounds__(256) void lin_slope_kernel(const T* __restrict__ dy
         part[(long)rb * N + cc] = t;
     }
 }
+// the column sums of the blocks, in order: 32 columns x 32 lanes of blocks
 template <class T>
-__global__ __launch_bounds__(256) void lin_bias_kernel(const float* __restrict__ part, int blocks, int N, T* __restrict__ db) {
-    __shared__ float sh[4][64];
-    const int cl = threadIdx.x & 63, q = threadIdx.x >> 6, c = blockIdx.x * 64 + cl;
+__global__ __launch_bounds__(1024) void lin_bias_kernel(const float* __restrict__ part, int blocks, int N, T* __restrict__ db) {
+    __shared__ float sh[32][33];
+    const int cl = threadIdx.x & 31, q = threadIdx.x >> 5, c = blockIdx.x * 32 + cl;
+    const float* at = part + (c < N ? c : N - 1);
     float s = 0.f;
-    if (c < N)
-        for (int b = q; b < blocks; b += 4) s += part[(long)b * N + c];
+#pragma unroll 4
+    for (int b = q; b < blocks; b += 32) s += at[(long)b * N];
     sh[q][cl] = s;
     __syncthreads();
-    if (q == 0 && c < N) st1(db[c], (sh[0][cl] + sh[1][cl]) + (sh[2][cl] + sh[3][cl]));
+    if (q || c >= N) return;
+#pragma unroll
+    for (int i = 1; i < 32; ++i) s += sh[i][cl];
+    st1(db[c], s);
 }
 
 long up8(long v) { return (v + 7) / 8 * 8; }
 bool al16(const void* p) { return ((size_t)p & 15) == 0; }
 size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 
-// Tile and splits of the sum over k.  256 x 256 tiles (one block a CU) where they alone fill the CUs; else 128 x 128 tiles (two a CU), and where those
-// leave most of the 512 slots empty the sum is split, a split keeping at least 256 of k.
-struct Plan { int bm, splits; };
+// Tile, slots and splits of the sum over k.
+struct Plan { int bm, slots, splits; };
 Plan plan(int M, int N, int K) {
-    const long big = ((M + 255L) / 256) * ((N + 255L) / 256), tiles = ((M + 127L) / 128) * ((N + 127L) / 128);
-    if (big >= 256) return {256, 1};
-    long s = 512 / (tiles > 0 ? tiles : 1);
+    auto tiles = [&](long t) { return ((M + t - 1) / t) * ((N + t - 1) / t); };
+    if (tiles(256) >= 256) return {256, 2, 1};
+    if (tiles(128) > 256) return {128, 2, 1};
+    if (tiles(128) >= 128) return {128, 4, 1};
+    if (tiles(64) >= 128 && K <= 2048) return {64, 4, 1};
+    const long t = tiles(128);
+    long s = 256 / t;
     if (s > K / 256) s = K / 256;
     if (s > 64) s = 64;
-    return {128, s < 1 ? 1 : (int)s};
+    return {128, 4, s < 1 ? 1 : (int)s};
 }
 size_t gemm_ws(int M, int N, int K) {
     const int s = plan(M, N, K).splits;
@@ -411,13 +509,13 @@ int prepare(const u16*& X, long& ldx, long rows, int cols, char*& ws, hipStream_
     return hipGetLastError() == hipSuccess ? 0 : cdae_fail("lin16: launch failed");
 }
 
-template <class T, bool AMC, bool BMC, int BM, int WN>
+template <class T, bool AMC, bool BMC, int BM, int WM, int WN, int SLOTS>
 int launch_tiles(const LinArgs& p, unsigned blocks, hipStream_t st) {
-    constexpr int smem = 2 * 2 * BM * 128;
-    auto* kernel = &lin_tile_kernel<T, AMC, BMC, BM, BM, 2, WN>;
+    constexpr int smem = SLOTS * 2 * BM * 128;
+    auto* kernel = &lin_tile_kernel<T, AMC, BMC, BM, BM, WM, WN, SLOTS>;
     if (smem > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, smem) != hipSuccess)
         return cdae_fail("lin16: hipFuncSetAttribute(max dynamic LDS) failed");
-    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(128 * WN), smem, st, p);
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * WM * WN), smem, st, p);
     return hipGetLastError() == hipSuccess ? 0 : cdae_fail("lin16: launch failed");
 }
 template <class T, bool AMC, bool BMC>
@@ -431,10 +529,15 @@ int product(LinArgs p, char* ws, hipStream_t st) {
     const long blocks = (long)p.tiles_m * p.tiles_n * p.splits;
     // (a lane's offset inside a stage is 32 bits: 256 rows, or 64 k rows and the columns)
     if (blocks > (1L << 22) || 512 * (AMC ? p.lda / 4 + p.M / 256 : p.lda) >= (1L << 32) || 512 * (BMC ? p.ldb / 4 + p.N / 256 : p.ldb) >= (1L << 32)) return cdae_fail("lin16: product too large");
-    if (pl.bm == 256 ? launch_tiles<T, AMC, BMC, 256, 4>(p, (unsigned)blocks, st) : launch_tiles<T, AMC, BMC, 128, 2>(p, (unsigned)blocks, st)) return -1;
+    const unsigned g = (unsigned)blocks;
+    if (pl.bm == 256 ? launch_tiles<T, AMC, BMC, 256, 2, 4, 2>(p, g, st)
+        : pl.bm == 64 ? launch_tiles<T, AMC, BMC, 64, 4, 1, 4>(p, g, st)
+        : pl.slots == 4 ? launch_tiles<T, AMC, BMC, 128, 2, 2, 4>(p, g, st)
+                        : launch_tiles<T, AMC, BMC, 128, 2, 2, 2>(p, g, st))
+        return -1;
     if (p.splits > 1) {
-        const long g = ((long)p.M * ((p.N + 7) / 8) + 255) / 256;
-        hipLaunchKernelGGL((lin_finish_kernel<T>), dim3((unsigned)(g < 8192 ? g : 8192)), dim3(256), 0, st, p);
+        const long f = ((long)p.M * ((p.N + 3) / 4) + 255) / 256;
+        hipLaunchKernelGGL((lin_finish_kernel<T>), dim3((unsigned)(f < 16384 ? f : 16384)), dim3(256), 0, st, p);
         if (hipGetLastError() != hipSuccess) return cdae_fail("lin16: launch failed");
     }
     return 0;
@@ -447,12 +550,19 @@ int bad_dims(int M, int N, int K, int dt) {
 }
 bool known_act(int a) { return a == L_NONE || a == L_SILU || a == L_RELU || a == L_GELU || a == L_GELU_TANH; }
 
-int slope_rows(int M, int N) {           // rows of a block of the slope pass: about 2048 blocks, at most 64 row blocks for the fold of the sums
+int slope_rows(int M, int N) {           // rows of a block of the slope pass: about 2048 blocks (eight a CU), 32 rows (four a thread) at least, 512 row blocks at most
     const int ncb = (N + 255) / 256;
     int rb = (2048 + ncb - 1) / ncb;
-    if (rb > 64) rb = 64;
-    int rows = (M + rb - 1) / rb;
-    return rows < 8 ? 8 : rows;
+    if (rb > 512) rb = 512;
+    const int rows = (int)(((long)M + rb - 1) / rb);
+    return rows < 32 ? 32 : (rows + 7) / 8 * 8;
+}
+template <class T>
+void slope_launch(const void* dy, long lddy, const void* z, long ldz, u16* dz, float* part, void* dbias, int M, int N, int act, hipStream_t st) {
+    const int ncb = (N + 255) / 256, rows = slope_rows(M, N), rb = (M + rows - 1) / rows;
+    auto* kernel = N < 8 ? &lin_slope_kernel<T, true> : &lin_slope_kernel<T, false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(ncb * rb)), dim3(256), 0, st, (const T*)dy, lddy, (const F16*)z, ldz, (T*)dz, up8(N), part, M, N, rows, ncb, act);
+    if (dbias) hipLaunchKernelGGL((lin_bias_kernel<T>), dim3((N + 31) / 32), dim3(1024), 0, st, part, rb, N, (T*)dbias);
 }
 
 }  // namespace
@@ -503,17 +613,9 @@ int cdae_lin16_bwd(const void* dy, long lddy, const void* x, long ldx, const voi
     u16* dz = nullptr;
     if (copy && (dx || dw)) { dz = (u16*)at; at += up256((size_t)M * up8(N) * 2); }
     if (dz || dbias) {
-        const int ncb = (N + 255) / 256, rows = slope_rows(M, N), rb = (M + rows - 1) / rows;
         float* part = dbias ? (float*)at : nullptr;
-        const dim3 grid((unsigned)(ncb * rb));
-        if (dt == DT_BF16)
-            hipLaunchKernelGGL((lin_slope_kernel<Bf16>), grid, dim3(256), 0, st, (const Bf16*)dy, lddy, (const _Float16*)z, ldz, (Bf16*)dz, up8(N), part, M, N, rows, ncb, act);
-        else
-            hipLaunchKernelGGL((lin_slope_kernel<F16>), grid, dim3(256), 0, st, (const F16*)dy, lddy, (const _Float16*)z, ldz, (F16*)dz, up8(N), part, M, N, rows, ncb, act);
-        if (dbias) {
-            if (dt == DT_BF16) hipLaunchKernelGGL((lin_bias_kernel<Bf16>), dim3((N + 63) / 64), dim3(256), 0, st, part, rb, N, (Bf16*)dbias);
-            else hipLaunchKernelGGL((lin_bias_kernel<F16>), dim3((N + 63) / 64), dim3(256), 0, st, part, rb, N, (F16*)dbias);
-        }
+        if (dt == DT_BF16) slope_launch<Bf16>(dy, lddy, z, ldz, dz, part, dbias, M, N, act, st);
+        else slope_launch<F16>(dy, lddy, z, ldz, dz, part, dbias, M, N, act, st);
         if (hipGetLastError() != hipSuccess) return cdae_fail("lin16_bwd: launch failed");
     }
     const u16* d = dz ? dz : (const u16*)dy;

@@ -3,6 +3,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "cdae_internal.h"
+
 enum { DT_BF16 = 0, DT_F16 = 1, DT_F32 = 2 };
 
 struct Bf16 { unsigned short u; };
@@ -57,3 +59,10 @@ __device__ __forceinline__ void st2(void* p, long off, int is32, float v) {
     if (is32) reinterpret_cast<float*>(p)[off] = v;
     else st1(reinterpret_cast<T*>(p)[off], v);
 }
+
+// a call's launches in the opt-in profiler (their family, flops or bytes of work, bytes that have to move)
+struct Timed {
+    const int family; const hipStream_t st;
+    Timed(int family_, double work, double bytes, hipStream_t st_) : family(family_), st(st_) { cdae_prof_begin(family, work, st); cdae_prof_note(family, bytes); }
+    ~Timed() { cdae_prof_end(family, st); }
+};

@@ -143,6 +143,12 @@ __global__ __launch_bounds__(256) void gc_scale_kernel(const GcTab t, long chunk
 
 int bytes_of(int ty) { return ty == DT_F32 ? 4 : 2; }
 
+double bytes_in(const long* n, const int* types, int count) {
+    double b = 0.0;
+    for (int i = 0; i < count; ++i) b += (double)n[i] * bytes_of(types[i]);
+    return b;
+}
+
 // The next table of a list: joins entries that lie back to back (in and out, same types), skips empty ones.  -> entries used from `at`
 int fill(GcTab& t, const void* const* in, const long* n, const int* types, void* const* out, const int* out_types, int count, int at, long& chunks) {
     t.count = 0;
@@ -239,6 +245,8 @@ int cdae_grad_norm(const void* const* in, const long* n, const int* types, int c
     if (!norm || !ws || ws_bytes < cdae_grad_workspace_bytes()) return cdae_fail("grad_norm: norm[2] and a workspace of cdae_grad_workspace_bytes() required");
     if (!(max_norm >= 0.0)) return cdae_fail("grad_norm: max_norm must be a number >= 0 (infinity: nothing is clipped)");
     hipStream_t st = (hipStream_t)stream;
+    const double bytes = bytes_in(n, types, count);
+    const Timed timed(PROF_OPT, bytes, bytes, st);
     double* slots = (double*)ws;
     const int used = launch_norm(in, n, types, count, slots, st);
     if (used < 0) return -1;
@@ -255,6 +263,8 @@ int cdae_grad_clip(const void* const* in, const long* n, const int* types, void*
     if (const int rc = check_overlap(in, n, types, out, out_types, count))
         return cdae_fail(rc == 1 ? "grad_clip: two outputs share memory, or an output shares memory with a gradient other than its own" : "grad_clip: out of host memory");
     hipStream_t st = (hipStream_t)stream;
+    const double bytes = bytes_in(n, types, count) + bytes_in(n, out_types, count);
+    const Timed timed(PROF_OPT, bytes, bytes, st);
     double* slots = (double*)ws;
     const int used = launch_norm(in, n, types, count, slots, st);
     if (used < 0) return -1;

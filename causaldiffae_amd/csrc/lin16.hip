@@ -8,6 +8,8 @@
 #include <hip/hip_runtime.h>
 #include <math.h>
 
+#include <atomic>
+#include <initializer_list>
 #include <type_traits>
 
 #include "cdae.h"
@@ -369,13 +371,16 @@ __global__ __launch_bounds__(256) void lin_finish_kernel(const LinArgs p) {
     }
 }
 
-// [rows][cols] at any pitch and alignment -> a dense image whose rows are padded with zeros to `pitch` (a multiple of 8)
-__global__ __launch_bounds__(256) void lin_pad_kernel(const u16* __restrict__ src, long lds_, u16* __restrict__ dst, long rows, int cols, int pitch) {
-    const long per = pitch / 8, total = per * rows;
+// [rows][cols] at any pitch and alignment -> dense rows padded with zeros to `pitch`, a multiple of 8; up to two operands in one launch
+struct PadJob { const u16* src; u16* dst; long ld, rows; int cols, pitch; };
+struct PadJobs { PadJob j[2]; };
+__global__ __launch_bounds__(256) void lin_pad_kernel(const PadJobs jobs) {
+    const PadJob p = jobs.j[blockIdx.y];
+    const long per = p.pitch / 8, total = per * p.rows;
     for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
         const long r = i / per;
-        const int c = (int)(i - r * per) * 8, have = cols - c;
-        const u16* s = src + r * lds_ + c;
+        const int c = (int)(i - r * per) * 8, have = p.cols - c;
+        const u16* s = p.src + r * p.ld + c;
         Pack<u16, 8> t;
         if (have >= 8) t = *reinterpret_cast<const Pack<u16, 8>*>(s);
         else
@@ -384,7 +389,7 @@ __global__ __launch_bounds__(256) void lin_pad_kernel(const u16* __restrict__ sr
         u32x4 w;
 #pragma unroll
         for (int e = 0; e < 4; ++e) w[e] = (unsigned)t.v[2 * e] | (unsigned)t.v[2 * e + 1] << 16;
-        *reinterpret_cast<u32x4*>(dst + r * pitch + c) = w;
+        *reinterpret_cast<u32x4*>(p.dst + r * p.pitch + c) = w;
     }
 }
 
@@ -477,35 +482,58 @@ long up8(long v) { return (v + 7) / 8 * 8; }
 bool al16(const void* p) { return ((size_t)p & 15) == 0; }
 size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 
-// Tile, slots and splits of the sum over k.
+// Tile, slots and splits of the sum over k: the cheapest by what a stage of 64 k and a tile's beginning and end cost (us), as measured on bf16 operands:
+//     256 x 256, one block a CU                    1.5   9      16384 x 2048 x 8192 weight gradient, 256 tiles of 256 stages: 384 us (128 x 128 532)
+//     128 x 128, four slots, one block a CU        0.5   3      8192 x 2048 -> 512 forward, 256 tiles of 32 stages: 19.3 us (two slots 24.3, 64 x 64 26.5)
+//     128 x 128, two slots, two blocks a CU        1.03  2.7    8192 x 384 -> 1536 forward, 768 tiles of 6 stages: 17.8 us (256 x 256 18.7, 64 x 64 24.1)
+//     64 x 64, one block a CU                      0.26  2.5    1024 x 392 -> 768 data gradient, 112 tiles of 12 stages: 6.3 us (128 x 128 10.7)
+//     64 x 64, two blocks a CU                     0.38  3.5    2048 x 1024 -> 1024 forward, 512 tiles of 16 stages: 8.4 us (128 x 128 11.4)
+// A split costs a second launch (3.5) and its partial sums twice (6 TB/s): 1536 x 384 over 8192 rows 26.8 us in seven splits, 64.1 in one, 36.5 in
+// fourteen; 2048 x 1024 over 1024 rows 11.2 in one, 16.8 in two.
 struct Plan { int bm, slots, splits; };
 Plan plan(int M, int N, int K) {
-    auto tiles = [&](long t) { return ((M + t - 1) / t) * ((N + t - 1) / t); };
-    if (tiles(256) >= 256) return {256, 2, 1};
-    if (tiles(128) > 256) return {128, 2, 1};
-    if (tiles(128) >= 128) return {128, 4, 1};
-    if (tiles(64) >= 128 && K <= 2048) return {64, 4, 1};
-    const long t = tiles(128);
-    long s = 256 / t;
-    if (s > K / 256) s = K / 256;
-    if (s > 64) s = 64;
-    return {128, 4, s < 1 ? 1 : (int)s};
+    struct Kind { int bm, slots, at_once; double stage, ends; };
+    static const Kind kinds[] = {{256, 2, 256, 1.5, 9.0}, {128, 4, 256, 0.5, 3.0}, {128, 2, 512, 1.03, 2.7}, {64, 4, 256, 0.26, 2.5}, {64, 4, 512, 0.38, 3.5}};
+    static const int splits[] = {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 28, 32, 48, 64};
+    const int only = cdae_tune(TUNE_LIN16_TILE), forced = cdae_tune(TUNE_LIN16_SPLITS);
+    Plan best{256, 2, 1};
+    double least = 1e30;
+    for (const Kind& k : kinds) {
+        if (only && (k.bm != kinds[only - 1].bm || k.slots != kinds[only - 1].slots)) continue;
+        const long tiles = ((M + k.bm - 1L) / k.bm) * ((N + k.bm - 1L) / k.bm);
+        if (tiles > (1L << 22)) continue;
+        for (int s : splits) {
+            if (forced ? s != forced : s > 1 && ((long)K / s < 256 || tiles * s > k.at_once)) continue;
+            const double rounds = (double)((tiles * s + k.at_once - 1) / k.at_once), stages = (double)(((K + s - 1) / s + 63) / 64);
+            const double cost = rounds * (stages * k.stage + k.ends) + (s > 1 ? 3.5 + 8.0 * s * M * N / 6e6 : 0.0);
+            if (cost < least) { least = cost; best = {k.bm, k.slots, s}; }
+        }
+    }
+    return best;
 }
 size_t gemm_ws(int M, int N, int K) {
     const int s = plan(M, N, K).splits;
     return s > 1 ? up256((size_t)s * M * N * 4) : 0;
 }
 
-// One operand in the form the tile kernel reads: 16-byte pieces, rows of a multiple of 8 values.  Copies it into `ws` where it is not.
-int prepare(const u16*& X, long& ldx, long rows, int cols, char*& ws, hipStream_t st) {
-    if (cols % 8 == 0 && ldx % 8 == 0 && al16(X)) return 0;
-    const long pitch = up8(cols);
-    u16* dst = (u16*)ws;
-    ws += up256((size_t)rows * pitch * 2);
-    const long total = rows * (pitch / 8);
-    const long g = (total + 255) / 256;
-    hipLaunchKernelGGL(lin_pad_kernel, dim3((unsigned)(g < 8192 ? g : 8192)), dim3(256), 0, st, X, ldx, dst, rows, cols, (int)pitch);
-    X = dst; ldx = pitch;
+// Operands in the form the tile kernel reads: 16-byte pieces, rows of a multiple of 8 values.  Those that are not are copied into `ws` by one launch.
+struct Operand { const u16** X; long* ldx; long rows; int cols; };
+int prepare(std::initializer_list<Operand> ops, char*& ws, hipStream_t st) {
+    PadJobs jobs{};
+    int n = 0;
+    long most = 0;
+    for (const Operand& o : ops) {
+        if (o.cols % 8 == 0 && *o.ldx % 8 == 0 && al16(*o.X)) continue;
+        const long pitch = up8(o.cols), pieces = o.rows * (pitch / 8);
+        u16* dst = (u16*)ws;
+        ws += up256((size_t)o.rows * pitch * 2);
+        jobs.j[n++] = {*o.X, dst, *o.ldx, o.rows, o.cols, (int)pitch};
+        *o.X = dst; *o.ldx = pitch;
+        if (pieces > most) most = pieces;
+    }
+    if (!n) return 0;
+    const long g = (most + 255) / 256;
+    hipLaunchKernelGGL(lin_pad_kernel, dim3((unsigned)(g < 8192 ? g : 8192), n), dim3(256), 0, st, jobs);
     return hipGetLastError() == hipSuccess ? 0 : cdae_fail("lin16: launch failed");
 }
 
@@ -513,8 +541,17 @@ template <class T, bool AMC, bool BMC, int BM, int WM, int WN, int SLOTS>
 int launch_tiles(const LinArgs& p, unsigned blocks, hipStream_t st) {
     constexpr int smem = SLOTS * 2 * BM * 128;
     auto* kernel = &lin_tile_kernel<T, AMC, BMC, BM, BM, WM, WN, SLOTS>;
-    if (smem > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, smem) != hipSuccess)
-        return cdae_fail("lin16: hipFuncSetAttribute(max dynamic LDS) failed");
+    if constexpr (smem > 65536) {                                         // once a device
+        static std::atomic<unsigned long long> done{0};
+        int dev = 0;
+        if (hipGetDevice(&dev) != hipSuccess) return cdae_fail("lin16: no device");
+        const unsigned long long bit = 1ull << (dev & 63);
+        if (!(done.load(std::memory_order_relaxed) & bit)) {
+            if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, smem) != hipSuccess)
+                return cdae_fail("lin16: hipFuncSetAttribute(max dynamic LDS) failed");
+            done.fetch_or(bit, std::memory_order_relaxed);
+        }
+    }
     hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * WM * WN), smem, st, p);
     return hipGetLastError() == hipSuccess ? 0 : cdae_fail("lin16: launch failed");
 }
@@ -575,8 +612,8 @@ size_t cdae_lin16_workspace_bytes(int op, int M, int N, int K) {
     if (op == CDAE_LIN16_FWD) return x + w + gemm_ws(M, N, K) + 256;
     if (op == CDAE_LIN16_BWD) {
         const int rows = slope_rows(M, N);
-        const size_t sums = up256(sizeof(float) * (size_t)N * ((M + rows - 1) / rows)), one = w + gemm_ws(M, K, N), two = x + gemm_ws(N, K, M);
-        const size_t most = one > two ? one : two;
+        const size_t sums = up256(sizeof(float) * (size_t)N * ((M + rows - 1) / rows)), one = gemm_ws(M, K, N), two = gemm_ws(N, K, M);
+        const size_t most = w + x + (one > two ? one : two);
         return d + (sums > most ? sums : most) + 256;
     }
     return 0;
@@ -590,10 +627,11 @@ int cdae_lin16_fwd(const void* x, long ldx, const void* w, long ldw, const void*
     if (!x || !w || !y || ldx < K || ldw < K || ldy < N || (res && ldres < N) || (z && ldz < N)) return cdae_fail("lin16_fwd: x, w, y and row pitches of at least a row required");
     if (ws_bytes < cdae_lin16_workspace_bytes(CDAE_LIN16_FWD, M, N, K) || !ws) return cdae_fail("lin16_fwd: workspace of cdae_lin16_workspace_bytes() required");
     hipStream_t st = (hipStream_t)stream;
+    const Timed timed(PROF_IGEMM, 2.0 * M * N * K, 2.0 * ((double)M * K + (double)N * K + (double)M * N * (1 + (res != nullptr) + (z != nullptr))), st);
     LinArgs p{};
     char* at = (char*)ws;
     p.A = (const u16*)x; p.lda = ldx; p.B = (const u16*)w; p.ldb = ldw;
-    if (prepare(p.A, p.lda, M, K, at, st) || prepare(p.B, p.ldb, N, K, at, st)) return -1;
+    if (prepare({{&p.A, &p.lda, M, K}, {&p.B, &p.ldb, N, K}}, at, st)) return -1;
     p.M = M; p.N = N; p.K = K;
     p.bias = (const u16*)bias; p.res = (const u16*)res; p.ldres = ldres; p.y = (u16*)y; p.ldy = ldy; p.z = (_Float16*)z; p.ldz = ldz; p.act = act;
     return dt == DT_BF16 ? product<Bf16, false, false>(p, at, st) : product<F16, false, false>(p, at, st);
@@ -608,6 +646,8 @@ int cdae_lin16_bwd(const void* dy, long lddy, const void* x, long ldx, const voi
     if ((dx && (!w || ldw < K || lddx < K)) || (dw && (!x || ldx < K || lddw < K))) return cdae_fail("lin16_bwd: w for dx, x for dw, row pitches of at least a row");
     if (!ws || ws_bytes < cdae_lin16_workspace_bytes(CDAE_LIN16_BWD, M, N, K)) return cdae_fail("lin16_bwd: workspace of cdae_lin16_workspace_bytes() required");
     hipStream_t st = (hipStream_t)stream;
+    const Timed timed(PROF_IGEMM, 2.0 * M * N * K * ((dx != nullptr) + (dw != nullptr)),
+                      2.0 * ((double)M * N * (act ? 2 : 1) + (double)M * K * ((dx != nullptr) + (dw != nullptr)) + (double)N * K * ((dx != nullptr) + (dw != nullptr))), st);
     char* at = (char*)ws;
     const bool copy = act != L_NONE || N % 8 || lddy % 8 || !al16(dy);
     u16* dz = nullptr;
@@ -620,24 +660,16 @@ int cdae_lin16_bwd(const void* dy, long lddy, const void* x, long ldx, const voi
     }
     const u16* d = dz ? dz : (const u16*)dy;
     const long ldd = dz ? up8(N) : lddy;
-    if (dx) {
-        LinArgs p{};
-        p.A = d; p.lda = ldd; p.B = (const u16*)w; p.ldb = ldw;
-        char* tmp = at;                                     // (a stream's launches run in order: the products use the same scratch one after the other)
-        if (prepare(p.B, p.ldb, N, K, tmp, st)) return -1;
-        p.M = M; p.N = K; p.K = N;
-        p.y = (u16*)dx; p.ldy = lddx;
-        if (dt == DT_BF16 ? product<Bf16, false, true>(p, tmp, st) : product<F16, false, true>(p, tmp, st)) return -1;
-    }
-    if (dw) {
-        LinArgs p{};
-        p.A = d; p.lda = ldd; p.B = (const u16*)x; p.ldb = ldx;
-        char* tmp = at;
-        if (prepare(p.B, p.ldb, M, K, tmp, st)) return -1;
-        p.M = N; p.N = K; p.K = M;
-        p.y = (u16*)dw; p.ldy = lddw;
-        if (dt == DT_BF16 ? product<Bf16, true, true>(p, tmp, st) : product<F16, true, true>(p, tmp, st)) return -1;
-    }
+    // (a stream's launches run in order: the sums of the bias and the products use the same scratch one after the other, but the copies stay)
+    LinArgs px{}, pw{};
+    px.A = pw.A = d; px.lda = pw.lda = ldd;
+    px.B = (const u16*)w; px.ldb = ldw; pw.B = (const u16*)x; pw.ldb = ldx;
+    px.M = M; px.N = K; px.K = N; px.y = (u16*)dx; px.ldy = lddx;
+    pw.M = N; pw.N = K; pw.K = M; pw.y = (u16*)dw; pw.ldy = lddw;
+    const Operand ow{&px.B, &px.ldb, N, K}, ox{&pw.B, &pw.ldb, M, K};
+    if (dx && dw ? prepare({ow, ox}, at, st) : dx ? prepare({ow}, at, st) : dw ? prepare({ox}, at, st) : 0) return -1;
+    if (dx && (dt == DT_BF16 ? product<Bf16, false, true>(px, at, st) : product<F16, false, true>(px, at, st))) return -1;
+    if (dw && (dt == DT_BF16 ? product<Bf16, true, true>(pw, at, st) : product<F16, true, true>(pw, at, st))) return -1;
     return 0;
 }
 

@@ -543,6 +543,8 @@ int cdae_resnorm_fwd(const cdae_resnorm* p, void* stream) {
     if (check(p)) return -1;
     if ((p->f && !p->r) || (p->pre && !p->u)) return cdae_fail("resnorm_fwd: r with a block output, u with a pre norm");
     hipStream_t st = (hipStream_t)stream;
+    const double rows = (double)p->B * p->T * p->C * (p->dt == DT_F32 ? 4 : 2);
+    const Timed timed(PROF_GN, rows * (1 + 2 * (p->f != nullptr) + (p->pre != 0)), rows * (1 + 2 * (p->f != nullptr) + (p->pre != 0)), st);
     if (p->dt == DT_F32) fwd<float>(p, st);
     else if (p->dt == DT_F16) fwd<F16>(p, st);
     else fwd<Bf16>(p, st);
@@ -560,6 +562,8 @@ int cdae_resnorm_bwd(const cdae_resnorm* p, void* stream) {
         return cdae_fail("resnorm_bwd: a gradient of a vector that is not there");
     if (!p->ws || p->ws_bytes < cdae_resnorm_workspace_bytes(p->B, p->T, p->C)) return cdae_fail("resnorm_bwd: workspace of cdae_resnorm_workspace_bytes() required");
     hipStream_t st = (hipStream_t)stream;
+    const double rows = (double)p->B * p->T * p->C * (p->dt == DT_F32 ? 4 : 2) * (1 + (p->f != nullptr) + (p->dr != nullptr) + (p->du != nullptr) + (p->dx != nullptr) + (p->df != nullptr));
+    const Timed timed(PROF_GN, rows, rows, st);
     if (p->dt == DT_F32) bwd<float>(p, st);
     else if (p->dt == DT_F16) bwd<F16>(p, st);
     else bwd<Bf16>(p, st);

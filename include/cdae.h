@@ -513,10 +513,14 @@ int cdae_rep_loss_bwd(const float* mu, const float* var, const float* z_post, co
  *                                      the step's pixels) where every member of a launch has Cout % 128 == 0: 1 = launches of two or more members,
  *                                      2 = every launch (tests), 0 = never
  *   CDAE_TUNE_WG16_SLOTS         (512) cdae_linear_wgrad_io's streaming kernel (wg16.hip) splits its rows until tiles x splits reach this many blocks
- *                                      (two block slots per CU = 512; half of it when dW has at most four tiles); fewer blocks = fewer, larger slabs for the finish */
+ *                                      (two block slots per CU = 512; half of it when dW has at most four tiles); fewer blocks = fewer, larger slabs for the finish
+ *   CDAE_TUNE_LIN16_TILE         (0)   products of cdae_lin16_*: 0 = the tile that their measured cost model finds cheapest; 1 = 256 x 256, 2 = 128 x 128 with four
+ *                                      slots, 3 = 128 x 128 with two, 4 = 64 x 64 (tests).  Workspace sizes follow it
+ *   CDAE_TUNE_LIN16_SPLITS       (0)   their split of the sum over k: 0 = by the same model, 1 .. 8 = that many (tests) */
 enum { CDAE_TUNE_CONVWIN_MIN_TILES = 0, CDAE_TUNE_CONVWIN_SPLITK = 1, CDAE_TUNE_CONVWIN_NJ3 = 2, CDAE_TUNE_HEAD_MFMA = 3, CDAE_TUNE_ROWS16_MIN_M = 4,
        CDAE_TUNE_ROWS16_RING = 5, CDAE_TUNE_CONVWIN_PAIR16 = 6, CDAE_TUNE_GN_BWD_FOLD2 = 7, CDAE_TUNE_GROUP_BIG_TILES = 8, CDAE_TUNE_CONVWIN_NJ2 = 9,
-       CDAE_TUNE_WGWIN_DIST = 10, CDAE_TUNE_WGWIN_SWZ = 11, CDAE_TUNE_WG16_SLOTS = 12, CDAE_TUNE_WGWIN_FIXED = 13, CDAE_TUNE_WGWIN_CO2 = 14 };
+       CDAE_TUNE_WGWIN_DIST = 10, CDAE_TUNE_WGWIN_SWZ = 11, CDAE_TUNE_WG16_SLOTS = 12, CDAE_TUNE_WGWIN_FIXED = 13, CDAE_TUNE_WGWIN_CO2 = 14, CDAE_TUNE_LIN16_TILE = 15,
+       CDAE_TUNE_LIN16_SPLITS = 16 };
 int cdae_tune_set(int key, int value);
 int cdae_tune_get(int key);       /* -1: unknown key */
 

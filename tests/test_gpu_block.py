@@ -109,6 +109,24 @@ def test_linear_act_sizes(M, K, N, dtype):
     check_linear(rnd(1, M, K, dtype=dtype), rnd(2, N, K, dtype=dtype, scale=K ** -0.5), rnd(3, N, dtype=dtype), res, act, rnd(5, M, N, dtype=dtype))
 
 
+@pytest.mark.parametrize("splits", [1, 2, 5])
+@pytest.mark.parametrize("tile", [1, 2, 3, 4])
+@pytest.mark.parametrize("M,K,N", [(300, 136, 520), (129, 1000, 65), (77, 393, 260), (513, 64, 8)])
+def test_linear_act_tiles(M, K, N, tile, splits):
+    """every tile and split at sizes inside one tile, on its edges and past them (by themselves such sizes take the small ones)"""
+    from causaldiffae_amd._lib import tune_scope
+    with tune_scope(lin16_tile=tile, lin16_splits=splits):
+        dtype = (BF16, F16)[tile % 2]
+        check_linear(rnd(1, M, K, dtype=dtype), rnd(2, N, K, dtype=dtype, scale=K ** -0.5), rnd(3, N, dtype=dtype), rnd(4, M, N, dtype=dtype), "gelu", rnd(5, M, N, dtype=dtype))
+
+
+def test_linear_act_large():
+    """sizes that take the large tiles by themselves, several rounds of them, against 64 bits"""
+    M, K, N = 4352, 1032, 4104
+    x, w, dy = rnd(1, M, K, dtype=BF16), rnd(2, N, K, dtype=BF16, scale=K ** -0.5), rnd(3, M, N, dtype=BF16)
+    check_linear(x, w, rnd(4, N, dtype=BF16), None, "none", dy)
+
+
 @pytest.mark.parametrize("act", list(ACT))
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_linear_act_activations(act, dtype):

@@ -35,6 +35,25 @@ __device__ __forceinline__ void stv(T* __restrict__ p, const float (&o)[V]) {
     for (int i = 0; i < V; ++i) st1(t.v[i], o[i]);
     *reinterpret_cast<Pack<T, V>*>(p) = t;
 }
+// Past the caches: data that is not read again soon.  (4-byte pieces of unaligned vectors: the instructions stay 16 bytes wide)
+typedef unsigned u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
+template <class P>
+__device__ __forceinline__ P load_past(const P* p) {
+    static_assert(sizeof(P) == 16, "one 16-byte piece");
+    return __builtin_bit_cast(P, __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(p)));
+}
+template <class P>
+__device__ __forceinline__ void store_past(P* p, const P& v) {
+    static_assert(sizeof(P) == 8 || sizeof(P) % 16 == 0, "whole pieces");
+    if constexpr (sizeof(P) == 8) __builtin_nontemporal_store(__builtin_bit_cast(u32x2_any, v), reinterpret_cast<u32x2_any*>(p));
+    else {
+        struct Pieces { u32x4_any q[sizeof(P) / 16]; };
+        const Pieces w = __builtin_bit_cast(Pieces, v);
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(P) / 16); ++i) __builtin_nontemporal_store(w.q[i], reinterpret_cast<u32x4_any*>(p) + i);
+    }
+}
 // the same with only the first n (0..V) values present; the others read as zero and are not written
 template <class T, int V>
 __device__ __forceinline__ void ldv_n(const T* __restrict__ p, int n, float (&o)[V]) {

@@ -83,6 +83,7 @@ struct LinArgs {
     const u16* bias; const u16* res; long ldres; u16* y; long ldy; _Float16* z; long ldz; int act;
     float* slab; int splits, k_per_split;   // splits > 1: partial sums [split][M][N] instead of the epilogue
     int tiles_m, tiles_n;
+    int past;                               // the result is larger than the caches: written past them
 };
 
 template <class T> struct Mfma;
@@ -108,7 +109,7 @@ __device__ __forceinline__ void finish_row(const LinArgs& p, long m, int n0, int
         Pack<F16, V> k;
 #pragma unroll
         for (int i = 0; i < V; ++i) k.v[i].h = (_Float16)v[i];
-        if (n >= V) *reinterpret_cast<Pack<F16, V>*>(zp) = k;
+        if (n >= V) store_past(reinterpret_cast<Pack<F16, V>*>(zp), k);    // (the backward reads it, long after)
         else
 #pragma unroll
             for (int i = 0; i < V; ++i) if (i < n) zp[i] = k.v[i].h;
@@ -119,7 +120,13 @@ __device__ __forceinline__ void finish_row(const LinArgs& p, long m, int n0, int
     if (p.res)
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] += ld1(r.v[i]);
-    stv_n<T, V>(reinterpret_cast<T*>(p.y) + m * p.ldy + n0, n, v);
+    T* const yp = reinterpret_cast<T*>(p.y) + m * p.ldy + n0;
+    if (n >= V && p.past) {
+        Pack<T, V> w;
+#pragma unroll
+        for (int i = 0; i < V; ++i) st1(w.v[i], v[i]);
+        store_past(reinterpret_cast<Pack<T, V>*>(yp), w);
+    } else stv_n<T, V>(yp, n, v);
 }
 // the residual of a row's n values (present ones only)
 template <class T, int V>
@@ -394,56 +401,45 @@ __global__ __launch_bounds__(256) void lin_pad_kernel(const PadJobs jobs) {
 }
 
 // dz = dy o act'(z) (written where wanted) and its column sums over a block's rows.  An HBM stream (three values of 2 bytes a result).  A block: 256
-// columns x 8 lanes of rows, 8 columns a thread, four rows in flight.  Loads and stores have no branches around them: the last thread of a row takes
-// the row's LAST 8 values (its neighbour's are among them, written twice with the same value and summed once), rows past the block's end repeat its last.
-// SMALL: rows of fewer than 8 values.
+// columns x 8 lanes of rows, 8 columns a thread, one row at a time (8192 x 1536 with GELU, sums only: 14.2 us; two rows in flight 15.9, four 17.7, eight
+// 29.3: the waves' number is worth more than their registers).  Loads and stores have no branches around them: the last thread of a row takes the row's
+// LAST 8 values (its neighbour's are among them, written twice with the same value and summed once).  SMALL: rows of fewer than 8 values.
 template <class T, bool SMALL>
 __global__ __launch_bounds__(256) void lin_slope_kernel(const T* __restrict__ dy, long lddy, const F16* __restrict__ z, long ldz, T* __restrict__ dz, long lddz,
                                                         float* __restrict__ part, int M, int N, int rows_per_block, int ncb, int act) {
-    constexpr int U = 4;
     __shared__ float sh[8][256];
     const int cb = blockIdx.x % ncb, rb = blockIdx.x / ncb;
     const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
     const int want = cb * 256 + cl * 8, c = SMALL ? 0 : want < N - 8 ? want : N - 8;
     const long r0 = (long)rb * rows_per_block, r1 = r0 + rows_per_block < M ? r0 + rows_per_block : M;
     float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (long r = r0 + rl; r < r1; r += 8 * U) {
-        Pack<T, 8> g[U];
-        Pack<F16, 8> k[U];
+    for (long r = r0 + rl; r < r1; r += 8) {
+        Pack<T, 8> g;
+        Pack<F16, 8> k;
+        if constexpr (SMALL) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const long rr = r + 8 * u < r1 ? r + 8 * u : r1 - 1;
-            if constexpr (SMALL) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) { g[u].v[e] = dy[rr * lddy + (e < N ? e : N - 1)]; if (act != L_NONE) k[u].v[e] = z[rr * ldz + (e < N ? e : N - 1)]; }
-            } else {
-                g[u] = *reinterpret_cast<const Pack<T, 8>*>(dy + rr * lddy + c);
-                if (act != L_NONE) k[u] = *reinterpret_cast<const Pack<F16, 8>*>(z + rr * ldz + c);
-            }
+            for (int e = 0; e < 8; ++e) { g.v[e] = dy[r * lddy + (e < N ? e : N - 1)]; if (act != L_NONE) k.v[e] = z[r * ldz + (e < N ? e : N - 1)]; }
+        } else {
+            g = *reinterpret_cast<const Pack<T, 8>*>(dy + r * lddy + c);
+            if (act != L_NONE) k = *reinterpret_cast<const Pack<F16, 8>*>(z + r * ldz + c);
         }
+        float v[8];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const bool live = r + 8 * u < r1;
-            const long rr = live ? r + 8 * u : r1 - 1;
-            float v[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = ld1(g[u].v[e]);
-#define LIN_CALL(A) _Pragma("unroll") for (int e = 0; e < 8; ++e) v[e] *= slope_of<A>(kept_z(k[u].v[e]))
-            LIN_ACT(act, LIN_CALL)
+        for (int e = 0; e < 8; ++e) v[e] = ld1(g.v[e]);
+#define LIN_CALL(A) _Pragma("unroll") for (int e = 0; e < 8; ++e) v[e] *= slope_of<A>(kept_z(k.v[e]))
+        LIN_ACT(act, LIN_CALL)
 #undef LIN_CALL
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s[e] += live ? v[e] : 0.f;
-            if (dz) {
-                if constexpr (SMALL) {
-                    if (cl == 0)
+        for (int e = 0; e < 8; ++e) s[e] += v[e];
+        if (!dz) continue;
+        if constexpr (SMALL) {
+            if (cl == 0)
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) st1(dz[rr * lddz + e], e < N ? v[e] : 0.f);
-                } else {
-                    stv<T, 8>(dz + rr * lddz + c, v);
-                    if (N & 7 && want <= N && want + 8 > N)                // the row's padding to a multiple of 8
-                        for (int e = N; e < lddz; ++e) st1(dz[rr * lddz + e], 0.f);
-                }
-            }
+                for (int e = 0; e < 8; ++e) st1(dz[r * lddz + e], e < N ? v[e] : 0.f);
+        } else {
+            stv<T, 8>(dz + r * lddz + c, v);
+            if (N & 7 && want <= N && want + 8 > N)                        // the row's padding to a multiple of 8
+                for (int e = N; e < lddz; ++e) st1(dz[r * lddz + e], 0.f);
         }
     }
     if (!part) return;
@@ -563,6 +559,8 @@ int product(LinArgs p, char* ws, hipStream_t st) {
     p.k_per_split = ((p.K + p.splits - 1) / p.splits + 63) / 64 * 64;
     p.splits = (p.K + p.k_per_split - 1) / p.k_per_split;
     p.slab = (float*)ws;
+    // (16384 x 2048 -> 8192 forward with GELU and its pre-activation kept: 534 us through the caches, 514 with the pre-activation past them, 490 with both)
+    p.past = (double)p.M * p.N * 2 > 64e6;
     const long blocks = (long)p.tiles_m * p.tiles_n * p.splits;
     // (a lane's offset inside a stage is 32 bits: 256 rows, or 64 k rows and the columns)
     if (blocks > (1L << 22) || 512 * (AMC ? p.lda / 4 + p.M / 256 : p.lda) >= (1L << 32) || 512 * (BMC ? p.ldb / 4 + p.N / 256 : p.ldb) >= (1L << 32)) return cdae_fail("lin16: product too large");

@@ -165,7 +165,7 @@ Tensor linear_act(const Tensor& x, const Tensor& w, const std::optional<Tensor>&
         for (int64_t i = 0; ok && i + 1 < x.dim(); ++i) ok = res.size(i) == x.size(i);
         REFUSE(ok, "linear_act: a residual of the result's shape (nothing is broadcast)");
     }
-    REFUSE(x.numel() / K < (1LL << 31) && N < (1LL << 31) && K < (1LL << 31), "linear_act: fewer than 2^31 rows");
+    REFUSE(x.numel() / K <= (1LL << 30) && N <= (1LL << 24) && K <= (1LL << 24), "linear_act: at most 2^30 rows and 2^24 features");
     c10::DeviceGuard on(x.device());
     if (wanted({x, w, b, res})) return LinearAct::apply(x, w, maybe(b), maybe(res), (int64_t)act);
     return linear_forward(rows_of(x, K), rows_of(w, K), b, res, act, nullptr, x);
@@ -288,7 +288,7 @@ py::tuple residual_norm(const Tensor& x, const std::optional<Tensor>& f_, const 
     REFUSE(type_of(x) >= 0, who, ": bf16, fp16 or fp32 rows (got ", x.scalar_type(), ")");
     REFUSE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= 8192, who, ": rows of 1 to 8192 features");
     const int64_t C = x.size(-1), M = x.numel() / C;
-    REFUSE(M < (1LL << 31), who, ": fewer than 2^31 rows");
+    REFUSE(M <= (1LL << 30), who, ": at most 2^30 rows");
     REFUSE(std::isfinite((float)alpha) && std::isfinite((float)eps) && eps >= 0, who, ": alpha finite, eps finite and not negative");
     REFUSE(!f.defined() || (f.sizes() == x.sizes() && f.scalar_type() == x.scalar_type()), who, ": f of x's shape and type");
     REFUSE(f.defined() || pre, who, ": without f there is only the pre norm to compute");

@@ -112,7 +112,7 @@ __device__ double total(const double* __restrict__ slots, int nslots) {
 __device__ __forceinline__ float clip_factor(double sum, double scale, double max_norm, float* norm) {
     const double n = sqrt(sum) * fabs(scale);
     *norm = (float)n;
-    const double c = max_norm / (n + 1e-6);
+    const double c = isinf(max_norm) ? 1.0 : max_norm / (n + 1e-6);
     return (float)(scale * (c >= 1.0 ? 1.0 : c));           // (a norm that is not a number stays one in the factor)
 }
 

@@ -154,7 +154,8 @@ __device__ __forceinline__ void lds_dma16_s(const void* base, unsigned off, unsi
 //     barrier a stage;
 //   * the fragments of the next 32 k are read from LDS while these 32 k run on the matrix cores (two register sets); reads, requests and products
 //     are interleaved by hand;
-//   * operand images: KC, rows of 128 bytes (whole cache lines: with 64-byte rows each line was fetched twice, 581 us for that product) whose
+//   * operand images: KC, rows of 128 bytes (whole cache lines: with 64-byte rows each line was fetched twice, 581 us for 16384 x 8192 x 2048 where the
+//     MC x MC product of the same size took 458) whose
 //     16-byte piece j lies at j ^ f(row); MC, planes of up to 128 columns whose k row's piece j lies at j ^ 2 g(k row), read through the transpose
 //     read.  f, g spread the rows that one read touches over all banks; the permutation is applied to the global address of the DMA lane;
 //   * the operands are swapped in the instruction (B in the A slot): a lane's four accumulators are four consecutive columns of one row;
@@ -326,6 +327,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void lin_tile_kernel(const LinArgs
         for (int a = 0; a < PR; ++a)
 #pragma unroll
             for (int b = 0; b < FB; ++b) *reinterpret_cast<f32x4*>(own + (16 * a + i16) * 256 + (((4 * b + q) ^ i16) * 16)) = acc[PR * h + a][b];
+        asm volatile("" ::: "memory");                                    // (other lanes' values: the wave's LDS accesses run in the order written)
 #pragma unroll 1
         for (int i = 0; i < 2 * PR; i += RB) {
             const int r0 = 8 * i + (lane >> 3);
@@ -347,6 +349,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void lin_tile_kernel(const LinArgs
                 }
             }
         }
+        asm volatile("" ::: "memory");
     }
 }
 
@@ -580,6 +583,7 @@ int product(LinArgs p, char* ws, hipStream_t st) {
 
 int bad_dims(int M, int N, int K, int dt) {
     if (M < 0 || N <= 0 || K <= 0) return cdae_fail("lin16: M >= 0, N >= 1 and K >= 1 required");
+    if (M > 1 << 30 || N > 1 << 24 || K > 1 << 24) return cdae_fail("lin16: at most 2^30 rows and 2^24 features");
     if (dt != DT_BF16 && dt != DT_F16) return cdae_fail("lin16: type 0 (bf16) or 1 (fp16)");
     return 0;
 }

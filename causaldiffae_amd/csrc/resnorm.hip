@@ -37,7 +37,7 @@ namespace {
 constexpr int RN_V = 8;                          // values of a row in one thread's registers
 constexpr int RN_MAX_C = 8192;                   // 1024 threads x 8
 constexpr long RN_MAX_GRID = 1 << 20;            // (a launch holds fewer than 2^32 threads: more rows than this are walked by the same blocks)
-constexpr long RN_MAX_FOLD = 1 << 21;            // samples x 32-column blocks of a backward call (the same bound)
+constexpr long RN_MAX_BLOCKS = 1 << 22;          // chunks of a backward call: 2^22 x 1024 threads would be the bound itself
 
 constexpr int RN_SUMS = 7;                       // of a sample: g A1, g A2, (1 + s) A3, (1 + s) A4, and the gradients of g, s, t
 
@@ -397,40 +397,43 @@ __global__ __launch_bounds__(block_of(TPR)) void rn_bwd_kernel(const RnArgs a) {
 template <class T>
 __global__ __launch_bounds__(1024) void rn_fold_kernel(const RnArgs a, float* __restrict__ sums) {
     const cdae_resnorm& p = a.p;
-    const int ncb = (p.C + 31) / 32;
-    const long b = blockIdx.x / ncb;
-    const int cl = threadIdx.x & 31, q = threadIdx.x >> 5, c = (int)(blockIdx.x - b * ncb) * 32 + cl;
+    const int ncb = (p.C + 31) / 32, cl = threadIdx.x & 31, q = threadIdx.x >> 5;
     __shared__ float sh[4][32][33];
-    float A[4] = {0.f, 0.f, 0.f, 0.f};
-    const float* part = p.ws + b * a.nch * 4 * p.C + (c < p.C ? c : p.C - 1);
+    for (long job = blockIdx.x; job < (long)p.B * ncb; job += gridDim.x) {        // (the block's: its barriers are met by every thread)
+        const long b = job / ncb;
+        const int c = (int)(job - b * ncb) * 32 + cl;
+        float A[4] = {0.f, 0.f, 0.f, 0.f};
+        const float* part = p.ws + b * a.nch * 4 * p.C + (c < p.C ? c : p.C - 1);
 #pragma unroll 4
-    for (int ch = q; ch < a.nch; ch += 32) {
+        for (int ch = q; ch < a.nch; ch += 32) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) A[j] += part[((long)ch * 4 + j) * p.C];
+            for (int j = 0; j < 4; ++j) A[j] += part[((long)ch * 4 + j) * p.C];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sh[j][q][cl] = A[j];
+        __syncthreads();
+        if (q < 4) {                                                      // the threads of q add sum q, in order
+            float s = 0.f;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) s += sh[q][i][cl];
+            sh[q][0][cl] = s;
+        }
+        __syncthreads();
+        if (q || c >= p.C) continue;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) A[j] = sh[j][0][cl];
+        auto vec = [&](const void* v, long off, int is32, float none) { return !v ? none : is32 ? ((const float*)v)[off] : ld1(((const T*)v)[off]); };
+        const float g = vec(p.gate, (p.shared_gate ? 0 : b * p.ld_gate) + c, p.vec32, 1.f) * p.alpha, s1 = 1.f + vec(p.scale, (p.shared_scale ? 0 : b * p.ld_scale) + c, p.vec32, 0.f);
+        const float w1 = vec(p.w1, c, p.w32, 1.f), b1 = vec(p.b1, c, p.w32, 0.f), w2 = vec(p.w2, c, p.w32, 1.f), b2 = vec(p.b2, c, p.w32, 0.f);
+        const float dg = p.alpha * (w1 * A[0] + b1 * A[1]), ds = w2 * A[2] + b2 * A[3];
+        if (p.dgate && !p.shared_gate) st2<T>(p.dgate, b * p.C + c, p.vec32, dg);
+        if (p.dscale && !p.shared_scale) st2<T>(p.dscale, b * p.C + c, p.vec32, ds);
+        if (p.dshift && !p.shared_shift) st2<T>(p.dshift, b * p.C + c, p.vec32, A[3]);
+        const float o[RN_SUMS] = {g * A[0], g * A[1], s1 * A[2], s1 * A[3], dg, ds, A[3]};
+#pragma unroll
+        for (int j = 0; j < RN_SUMS; ++j) sums[(b * RN_SUMS + j) * p.C + c] = o[j];
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) sh[j][q][cl] = A[j];
-    __syncthreads();
-    if (q < 4) {                                                          // wave pair q of a block adds sum q, in order
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) s += sh[q][i][cl];
-        sh[q][0][cl] = s;
-    }
-    __syncthreads();
-    if (q || c >= p.C) return;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) A[j] = sh[j][0][cl];
-    auto vec = [&](const void* v, long off, int is32, float none) { return !v ? none : is32 ? ((const float*)v)[off] : ld1(((const T*)v)[off]); };
-    const float g = vec(p.gate, (p.shared_gate ? 0 : b * p.ld_gate) + c, p.vec32, 1.f) * p.alpha, s1 = 1.f + vec(p.scale, (p.shared_scale ? 0 : b * p.ld_scale) + c, p.vec32, 0.f);
-    const float w1 = vec(p.w1, c, p.w32, 1.f), b1 = vec(p.b1, c, p.w32, 0.f), w2 = vec(p.w2, c, p.w32, 1.f), b2 = vec(p.b2, c, p.w32, 0.f);
-    const float dg = p.alpha * (w1 * A[0] + b1 * A[1]), ds = w2 * A[2] + b2 * A[3];
-    if (p.dgate && !p.shared_gate) st2<T>(p.dgate, (long)b * p.C + c, p.vec32, dg);
-    if (p.dscale && !p.shared_scale) st2<T>(p.dscale, (long)b * p.C + c, p.vec32, ds);
-    if (p.dshift && !p.shared_shift) st2<T>(p.dshift, (long)b * p.C + c, p.vec32, A[3]);
-    const float o[RN_SUMS] = {g * A[0], g * A[1], s1 * A[2], s1 * A[3], dg, ds, A[3]};
-#pragma unroll
-    for (int j = 0; j < RN_SUMS; ++j) sums[((long)b * RN_SUMS + j) * p.C + c] = o[j];
 }
 
 // what all samples share: grid y picks one of the seven sums; 32 columns x 8 lanes of samples
@@ -481,7 +484,7 @@ void fwd_chunks(int B, int T, int C, int& nch, int& rows) {
 
 int check(const cdae_resnorm* p) {
     if (!p || p->B <= 0 || p->T <= 0 || p->C <= 0 || p->C > RN_MAX_C) return cdae_fail("resnorm: B, T >= 1 and 1 <= C <= 8192 required");
-    if ((long)p->B * p->T > 0x7fffffffL) return cdae_fail("resnorm: at most 2^31 - 1 rows");
+    if ((long)p->B * p->T > 1L << 30) return cdae_fail("resnorm: at most 2^30 rows");
     if (p->dt < 0 || p->dt > 2) return cdae_fail("resnorm: row type 0 (bf16), 1 (fp16) or 2 (fp32)");
     if (!p->x || (!p->f && !p->pre)) return cdae_fail("resnorm: x and a block output or a pre norm required");
     if (!p->f && (p->post || p->gate)) return cdae_fail("resnorm: a post norm or a gate needs a block output");
@@ -525,7 +528,8 @@ void bwd(const cdae_resnorm* p, hipStream_t st) {
     RN_TPR(RN_CALL)
 #undef RN_CALL
     if (!(p->dgate || p->dscale || p->dshift || p->dw1 || p->db1 || p->dw2 || p->db2)) return;
-    hipLaunchKernelGGL((rn_fold_kernel<T>), dim3((unsigned)((p->C + 31) / 32 * (long)p->B)), dim3(1024), 0, st, a, sums);
+    const long jobs = (p->C + 31L) / 32 * p->B;
+    hipLaunchKernelGGL((rn_fold_kernel<T>), dim3((unsigned)(jobs < RN_MAX_GRID ? jobs : RN_MAX_GRID)), dim3(1024), 0, st, a, sums);
     if (p->dw1 || p->db1 || p->dw2 || p->db2 || (p->dgate && p->shared_gate) || (p->dscale && p->shared_scale) || (p->dshift && p->shared_shift))
         hipLaunchKernelGGL((rn_shared_kernel<T>), dim3((p->C + 31) / 32, RN_SUMS), dim3(256), 0, st, a, sums);
 }
@@ -555,7 +559,7 @@ int cdae_resnorm_fwd(const cdae_resnorm* p, void* stream) {
 
 int cdae_resnorm_bwd(const cdae_resnorm* p, void* stream) {
     if (check(p)) return -1;
-    if ((long)p->B * ((p->C + 31) / 32) > RN_MAX_FOLD) return cdae_fail("resnorm_bwd: at most 2^21 / ceil(C / 32) samples");
+    if (p->B >= RN_MAX_BLOCKS) return cdae_fail("resnorm_bwd: fewer than 2^22 samples");
     if (!p->dr && !p->du) return cdae_fail("resnorm_bwd: the gradient of r or of u required");
     if (p->du && !p->pre) return cdae_fail("resnorm_bwd: the gradient of u without a pre norm");
     if (!p->f && (p->df || p->dgate || p->dw1 || p->db1)) return cdae_fail("resnorm_bwd: gradients of a block output that is not there");

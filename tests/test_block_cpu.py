@@ -35,6 +35,9 @@ def test_linear_refusals():
     for kw in (dict(M=-1), dict(N=0), dict(K=0)):
         refused(fwd(**kw), "required")
         refused(bwd(**kw), "required")
+    for kw in (dict(M=(1 << 30) + 1), dict(N=(1 << 24) + 1), dict(K=(1 << 24) + 1)):
+        refused(fwd(**kw), "at most")
+        refused(bwd(**kw), "at most")
     refused(fwd(dt=2), "type")
     refused(bwd(dt=3), "type")
     for a in (2, 4, 7, -1):
@@ -79,7 +82,7 @@ def test_norm_refusals():
     refused(lib.cdae_resnorm_bwd(args(df=PTR), None), "not there")
     refused(lib.cdae_resnorm_bwd(args(dscale=PTR), None), "not there")
     refused(lib.cdae_resnorm_bwd(args(ws_bytes=16), None), "workspace")
-    refused(lib.cdae_resnorm_bwd(args(B=1 << 18, C=8192, T=1, ws_bytes=1 << 60), None), "samples")
+    refused(lib.cdae_resnorm_bwd(args(B=1 << 22, C=1, T=1), None), "samples")
 
 
 def test_grad_refusals():

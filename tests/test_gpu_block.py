@@ -401,6 +401,13 @@ def test_residual_norm_constant_and_huge_rows():
     check_norm(x, f, v, 1.0, False, True, "layer", dr=rnd(3, 1, 6, C), du=rnd(4, 1, 6, C))
 
 
+def test_residual_norm_many_samples():
+    """a vector for every row, more samples than one pass of the folding blocks' lanes"""
+    v = vectors(5000, 24, BF16, "sample", "sample", False, True)
+    r = lambda s: rnd(s, 5000, 24, dtype=BF16)
+    check_norm(r(1), r(2), v, 1.0, False, True, "layer", dr=r(3), du=r(4), shape=(5000, 1, 24))
+
+
 def test_residual_norm_no_rows():
     x = torch.empty(0, 5, 16, dtype=BF16, device=DEV).requires_grad_(True)
     w = rnd(1, 16, dtype=BF16).requires_grad_(True)
@@ -478,6 +485,11 @@ def test_clip_leaves_small_gradients_alone():
     assert abs(float(n) - exact_norm(keep)) <= 2 * u * float(n) and all(torch.equal(a, b) for a, b in zip(grads, keep))
     blk().clip_grad_norm_(grads, 0.0)
     assert all(not g.any() for g in grads)
+    g = rnd(1, 70)
+    g[3] = float("inf")
+    k = g.clone()
+    blk().clip_grad_norm_([g], math.inf)                        # nothing is clipped, whatever the norm
+    assert torch.equal(g, k)
 
 
 def test_clip_strides():

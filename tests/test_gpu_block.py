@@ -741,3 +741,53 @@ def test_train_loop_clips():
     assert exact_norm([c.opt.m]) == pytest.approx(0.0125, rel=1e-4)
     with pytest.raises(ValueError):
         TrainLoop(model=None, diffusion=None, data=None, batch_size=1, microbatch=1, lr=0.0, ema_rate="0", log_interval=1, save_interval=1, resume_checkpoint="", grad_clip=-1.0)
+
+
+# ----------------------------------------------------------------------------- offsets beyond 32 bits
+def tail_of(rows, C, seed, dtype=BF16, last=300):
+    """[rows, C] zeros whose last rows are not"""
+    t = torch.zeros(rows, C, dtype=dtype, device=DEV)
+    t[-last:] = rnd(seed, last, C, dtype=dtype)
+    return t
+
+
+def test_linear_act_long():
+    """2.3 billion values in and out: the last rows are those of a call on them alone, and so are the sums when only they have a gradient"""
+    M, C = (1 << 24) + 3, 136
+    x, w, b = tail_of(M, C, 1), rnd(2, C, C, dtype=BF16, scale=0.1), rnd(3, C, dtype=BF16)
+    xs = x[-300:].clone().requires_grad_(True)
+    x, w, b = (t.requires_grad_(True) for t in (x, w, b))
+    y, ys = blk().linear_act(x, w, b, act="silu"), blk().linear_act(xs, w, b, act="silu")
+    assert torch.equal(y[-300:], ys) and torch.equal(y[0], blk().linear_act(torch.zeros_like(xs[:1]), w, b, act="silu")[0])
+    dy = tail_of(M, C, 4)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    ref = linear_reference(xs.detach(), w.detach(), b.detach(), None, "silu", dy[-300:])
+    within("dx", dx[-300:], *ref["dx"])
+    assert not dx[:-300].any()
+    within("dw", dw, *ref["dw"])
+    within("db", db, *ref["db"])
+
+
+def test_residual_norm_long():
+    M, C = (1 << 22) + 1, 520
+    x, f, dr, du = (tail_of(M, C, i) for i in range(4))
+    v = vectors(1, C, BF16, "channel", "channel", True, True)
+    leaves = [t.requires_grad_(True) for t in (x, f, *v.values())]
+    call = lambda x, f: blk().residual_norm(x, f, gate=v["gate"], post=(v["w1"], v["b1"]), pre=(v["w2"], v["b2"]), scale=v["scale"], shift=v["shift"])
+    r, uu = call(x, f)
+    rs, us = call(x[-300:].detach(), f[-300:].detach())
+    assert torch.equal(r[-300:], rs) and torch.equal(uu[-300:], us)
+    got = torch.autograd.grad([r, uu], leaves, [dr, du])
+    t = {k: a.detach() for k, a in v.items()}
+    ref = norm_reference(x[-300:][None].detach(), f[-300:][None].detach(), t, 1.0, True, True, "layer", 1e-5, dr[-300:][None], du[-300:][None])
+    for k, g in zip(["x", "f", *v], got):
+        within("d" + k, g[-300:][None] if k in "xf" else g, *ref["d" + k])
+    assert not got[0][:-300].any() and not got[1][:-300].any()
+
+
+def test_clip_long():
+    g = torch.zeros((1 << 31) + 20001, dtype=BF16, device=DEV)
+    g[-1], g[5] = 3.0, 4.0
+    assert float(blk().grad_norm([g])) == 5.0
+    assert float(blk().clip_grad_norm_([g], 2.5)) == 5.0
+    assert float(g[-1]) == 1.5 and float(g[5]) == 2.0

@@ -161,16 +161,15 @@ __device__ __forceinline__ void lds_dma16_s(const void* base, unsigned off, unsi
 //   * the operands are swapped in the instruction (B in the A slot): a lane's four accumulators are four consecutive columns of one row;
 //   * blocks that run on one XCD (block number mod 8) take neighbouring tiles, 8 rows of tiles at a time: an operand's panel is read from HBM once an XCD.
 template <class T, bool AMC, bool BMC, int BM, int BN, int WM, int WN, int SLOTS>
-__global__ __launch_bounds__(64 * WM * WN, 2) void lin_tile_kernel(const LinArgs p) {
+__device__ __forceinline__ void lin_tile(const LinArgs& p, const int block, unsigned char* const lds) {
     constexpr int TM = BM / WM, TN = BN / WN, FA = TM / 16, FB = TN / 16;                 // a wave's part and its fragments
     constexpr int AB = BM * 128, STAGE = (BM + BN) * 128, DMAS = STAGE / (1024 * WM * WN);  // bytes of a stage's images; DMAs of 1 KB a wave
     constexpr int PA = BM < 128 ? BM : 128, PB = BN < 128 ? BN : 128;                     // columns of an MC plane
     static_assert(TN == 64 && AB / 1024 % DMAS == 0 && PA == PB, "64 columns a wave; a wave's DMAs belong to one operand");
-    extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i16 = lane & 15, q = lane >> 4;
     const int tiles = p.tiles_m * p.tiles_n;
-    const int split = blockIdx.x / tiles, id = blockIdx.x - split * tiles;
+    const int split = block / tiles, id = block - split * tiles;
     int tm, tn;
     {
         const int x = id & 7, per = tiles >> 3, more = tiles & 7;
@@ -352,6 +351,20 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void lin_tile_kernel(const LinArgs
         asm volatile("" ::: "memory");
     }
 }
+template <class T, bool AMC, bool BMC, int BM, int WM, int WN, int SLOTS>
+__global__ __launch_bounds__(64 * WM * WN, 2) void lin_tile_kernel(const LinArgs p) {
+    extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+    lin_tile<T, AMC, BMC, BM, BM, WM, WN, SLOTS>(p, blockIdx.x, lds);
+}
+// Both products of a backward pass in one launch: the weight gradient's blocks, then (from a multiple of 8, for the XCDs) the data gradient's.  Each alone
+// leaves CUs without work at its end, or from the beginning.
+template <class T, int BM, int WM, int WN, int SLOTS>
+__global__ __launch_bounds__(64 * WM * WN, 2) void lin_pair_kernel(const LinArgs pw, const LinArgs px, const int blocks_w) {
+    extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+    const int second = (blocks_w + 7) & ~7, block = blockIdx.x;
+    if (block < blocks_w) lin_tile<T, true, true, BM, BM, WM, WN, SLOTS>(pw, block, lds);
+    else if (block >= second) lin_tile<T, false, true, BM, BM, WM, WN, SLOTS>(px, block - second, lds);
+}
 
 // partial sums of the splits, added in order, then the epilogue: 4 columns a thread, eight splits in flight
 template <class T>
@@ -489,30 +502,65 @@ size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 //     64 x 64, two blocks a CU                     0.38  3.5    2048 x 1024 -> 1024 forward, 512 tiles of 16 stages: 8.4 us (128 x 128 11.4)
 // A split costs a second launch (3.5) and its partial sums twice (6 TB/s): 1536 x 384 over 8192 rows 26.8 us in seven splits, 64.1 in one, 36.5 in
 // fourteen; 2048 x 1024 over 1024 rows 11.2 in one, 16.8 in two.
-struct Plan { int bm, slots, splits; };
+struct Kind { int bm, slots, at_once; double stage, ends; };
+const Kind kinds[] = {{256, 2, 256, 1.5, 9.0}, {128, 4, 256, 0.5, 3.0}, {128, 2, 512, 1.03, 2.7}, {64, 4, 256, 0.26, 2.5}, {64, 4, 512, 0.38, 3.5}};
+bool kind_allowed(const Kind& k) {
+    const int only = cdae_tune(TUNE_LIN16_TILE);
+    return !only || (k.bm == kinds[only - 1].bm && k.slots == kinds[only - 1].slots);
+}
+long tiles_of(const Kind& k, int M, int N) { return ((M + k.bm - 1L) / k.bm) * ((N + k.bm - 1L) / k.bm); }
+double block_cost(const Kind& k, int K, int s) { return (double)(((K + s - 1) / s + 63) / 64) * k.stage + k.ends; }
+double split_cost(int M, int N, int s) { return s > 1 ? 3.5 + 8.0 * s * M * N / 6e6 : 0.0; }
+bool split_allowed(int K, int s) {
+    const int forced = cdae_tune(TUNE_LIN16_SPLITS);
+    return forced ? s == forced : s == 1 || K / s >= 256;
+}
+size_t slab_of(int M, int N, int s) { return s > 1 ? up256((size_t)s * M * N * 4) : 0; }
+
+struct Plan { int bm, slots, splits; double cost; };
 Plan plan(int M, int N, int K) {
-    struct Kind { int bm, slots, at_once; double stage, ends; };
-    static const Kind kinds[] = {{256, 2, 256, 1.5, 9.0}, {128, 4, 256, 0.5, 3.0}, {128, 2, 512, 1.03, 2.7}, {64, 4, 256, 0.26, 2.5}, {64, 4, 512, 0.38, 3.5}};
     static const int splits[] = {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 28, 32, 48, 64};
-    const int only = cdae_tune(TUNE_LIN16_TILE), forced = cdae_tune(TUNE_LIN16_SPLITS);
-    Plan best{256, 2, 1};
-    double least = 1e30;
+    Plan best{256, 2, 1, 1e30};
     for (const Kind& k : kinds) {
-        if (only && (k.bm != kinds[only - 1].bm || k.slots != kinds[only - 1].slots)) continue;
-        const long tiles = ((M + k.bm - 1L) / k.bm) * ((N + k.bm - 1L) / k.bm);
-        if (tiles > (1L << 22)) continue;
+        const long tiles = tiles_of(k, M, N);
+        if (!kind_allowed(k) || tiles > (1L << 22)) continue;
         for (int s : splits) {
-            if (forced ? s != forced : s > 1 && ((long)K / s < 256 || tiles * s > k.at_once)) continue;
-            const double rounds = (double)((tiles * s + k.at_once - 1) / k.at_once), stages = (double)(((K + s - 1) / s + 63) / 64);
-            const double cost = rounds * (stages * k.stage + k.ends) + (s > 1 ? 3.5 + 8.0 * s * M * N / 6e6 : 0.0);
-            if (cost < least) { least = cost; best = {k.bm, k.slots, s}; }
+            if (!split_allowed(K, s) || (s > 1 && tiles * s > k.at_once && !cdae_tune(TUNE_LIN16_SPLITS))) continue;
+            const double rounds = (double)((tiles * s + k.at_once - 1) / k.at_once), cost = rounds * block_cost(k, K, s) + split_cost(M, N, s);
+            if (cost < best.cost) best = {k.bm, k.slots, s, cost};
         }
     }
     return best;
 }
-size_t gemm_ws(int M, int N, int K) {
-    const int s = plan(M, N, K).splits;
-    return s > 1 ? up256((size_t)s * M * N * 4) : 0;
+// A backward's two products: dx [M][K] over N, dw [N][K] over M, each by its own plan, or together on one kind of tile where that is cheaper by the same
+// model (a launch that keeps all slots busy takes its blocks' time over the slots, and half a block for its end).
+// 8192 x 384 -> 1536: 36 us together, 49 one after the other (traced).
+struct Pair { bool together; int bm, slots, sx, sw; };
+Pair pair_plan(int M, int N, int K) {
+    static const int splits[] = {1, 2, 3, 4, 6, 8, 12, 16};
+    Pair best{false, 0, 0, 1, 1};
+    double least = plan(M, K, N).cost + plan(N, K, M).cost + 2.5;
+    for (const Kind& k : kinds) {
+        const long tx = tiles_of(k, M, K), tw = tiles_of(k, N, K);
+        if (!kind_allowed(k) || tx + tw > (1L << 21)) continue;
+        for (int sx : splits) {
+            if (!split_allowed(N, sx)) continue;
+            const double cx = block_cost(k, N, sx), ex = split_cost(M, K, sx);
+            for (int sw : splits) {
+                if (!split_allowed(M, sw)) continue;
+                const double cw = block_cost(k, M, sw), longest = cx > cw ? cx : cw, busy = ((double)tx * sx * cx + (double)tw * sw * cw) / k.at_once;
+                const double cost = (tx * sx + tw * sw <= k.at_once ? longest : busy + 0.5 * longest) + ex + split_cost(N, K, sw);
+                if (cost < least) { least = cost; best = {true, k.bm, k.slots, sx, sw}; }
+            }
+        }
+    }
+    return best;
+}
+size_t bwd_ws(int M, int N, int K) {
+    const Pair b = pair_plan(M, N, K);
+    const size_t x = slab_of(M, K, plan(M, K, N).splits), w = slab_of(N, K, plan(N, K, M).splits), one = x > w ? x : w;
+    const size_t both = b.together ? slab_of(M, K, b.sx) + slab_of(N, K, b.sw) : 0;
+    return one > both ? one : both;                                       // (a call may want one product only)
 }
 
 // Operands in the form the tile kernel reads: 16-byte pieces, rows of a multiple of 8 values.  Those that are not are copied into `ws` by one launch.
@@ -536,49 +584,84 @@ int prepare(std::initializer_list<Operand> ops, char*& ws, hipStream_t st) {
     return hipGetLastError() == hipSuccess ? 0 : cdae_fail("lin16: launch failed");
 }
 
-template <class T, bool AMC, bool BMC, int BM, int WM, int WN, int SLOTS>
-int launch_tiles(const LinArgs& p, unsigned blocks, hipStream_t st) {
-    constexpr int smem = SLOTS * 2 * BM * 128;
-    auto* kernel = &lin_tile_kernel<T, AMC, BMC, BM, BM, WM, WN, SLOTS>;
-    if constexpr (smem > 65536) {                                         // once a device
-        static std::atomic<unsigned long long> done{0};
-        int dev = 0;
-        if (hipGetDevice(&dev) != hipSuccess) return cdae_fail("lin16: no device");
-        const unsigned long long bit = 1ull << (dev & 63);
-        if (!(done.load(std::memory_order_relaxed) & bit)) {
-            if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, smem) != hipSuccess)
-                return cdae_fail("lin16: hipFuncSetAttribute(max dynamic LDS) failed");
-            done.fetch_or(bit, std::memory_order_relaxed);
-        }
+// dynamic LDS beyond 64 KB has to be asked for, once a device and kernel (`done`: its devices)
+int allow_lds(const void* kernel, int bytes, std::atomic<unsigned long long>& done) {
+    if (bytes <= 65536) return 0;
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) return cdae_fail("lin16: no device");
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (done.load(std::memory_order_relaxed) & bit) return 0;
+    if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return cdae_fail("lin16: hipFuncSetAttribute(max dynamic LDS) failed");
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return 0;
+}
+// a product's tiles and splits for tiles of bm; -> blocks, or -1
+template <bool AMC, bool BMC>
+long lay_out(LinArgs& p, int bm, int splits, char* slab) {
+    p.tiles_m = (p.M + bm - 1) / bm; p.tiles_n = (p.N + bm - 1) / bm;
+    p.k_per_split = ((p.K + splits - 1) / splits + 63) / 64 * 64;
+    p.splits = (p.K + p.k_per_split - 1) / p.k_per_split;
+    p.slab = (float*)slab;
+    // (16384 x 2048 -> 8192 forward with GELU and its pre-activation kept: 534 us through the caches, 514 with the pre-activation past them, 490 with both)
+    p.past = (double)p.M * p.N * 2 > 64e6;
+    const long blocks = (long)p.tiles_m * p.tiles_n * p.splits;
+    // (a lane's offset inside a stage is 32 bits: 256 rows, or 64 k rows and the columns)
+    if (blocks > (1L << 22) || 512 * (AMC ? p.lda / 4 + p.M / 256 : p.lda) >= (1L << 32) || 512 * (BMC ? p.ldb / 4 + p.N / 256 : p.ldb) >= (1L << 32)) {
+        cdae_fail("lin16: product too large");
+        return -1;
     }
-    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * WM * WN), smem, st, p);
+    return blocks;
+}
+template <class T>
+int finish(const LinArgs& p, hipStream_t st) {
+    if (p.splits <= 1) return 0;
+    const long f = ((long)p.M * ((p.N + 3) / 4) + 255) / 256;
+    hipLaunchKernelGGL((lin_finish_kernel<T>), dim3((unsigned)(f < 16384 ? f : 16384)), dim3(256), 0, st, p);
+    return hipGetLastError() == hipSuccess ? 0 : cdae_fail("lin16: launch failed");
+}
+template <class T, bool AMC, bool BMC, int BM, int WM, int WN, int SLOTS>
+int launch_tiles(const LinArgs& p, long blocks, hipStream_t st) {
+    constexpr int smem = SLOTS * 2 * BM * 128;
+    static std::atomic<unsigned long long> done{0};
+    auto* kernel = &lin_tile_kernel<T, AMC, BMC, BM, WM, WN, SLOTS>;
+    if (allow_lds(reinterpret_cast<const void*>(kernel), smem, done)) return -1;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * WM * WN), smem, st, p);
+    return hipGetLastError() == hipSuccess ? 0 : cdae_fail("lin16: launch failed");
+}
+template <class T, int BM, int WM, int WN, int SLOTS>
+int launch_pair(const LinArgs& pw, const LinArgs& px, long blocks_w, long blocks_x, hipStream_t st) {
+    constexpr int smem = SLOTS * 2 * BM * 128;
+    static std::atomic<unsigned long long> done{0};
+    auto* kernel = &lin_pair_kernel<T, BM, WM, WN, SLOTS>;
+    if (allow_lds(reinterpret_cast<const void*>(kernel), smem, done)) return -1;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((blocks_w + 7) / 8 * 8 + blocks_x)), dim3(64 * WM * WN), smem, st, pw, px, (int)blocks_w);
     return hipGetLastError() == hipSuccess ? 0 : cdae_fail("lin16: launch failed");
 }
 template <class T, bool AMC, bool BMC>
 int product(LinArgs p, char* ws, hipStream_t st) {
     const Plan pl = plan(p.M, p.N, p.K);
-    p.tiles_m = (p.M + pl.bm - 1) / pl.bm; p.tiles_n = (p.N + pl.bm - 1) / pl.bm;
-    p.splits = pl.splits;
-    p.k_per_split = ((p.K + p.splits - 1) / p.splits + 63) / 64 * 64;
-    p.splits = (p.K + p.k_per_split - 1) / p.k_per_split;
-    p.slab = (float*)ws;
-    // (16384 x 2048 -> 8192 forward with GELU and its pre-activation kept: 534 us through the caches, 514 with the pre-activation past them, 490 with both)
-    p.past = (double)p.M * p.N * 2 > 64e6;
-    const long blocks = (long)p.tiles_m * p.tiles_n * p.splits;
-    // (a lane's offset inside a stage is 32 bits: 256 rows, or 64 k rows and the columns)
-    if (blocks > (1L << 22) || 512 * (AMC ? p.lda / 4 + p.M / 256 : p.lda) >= (1L << 32) || 512 * (BMC ? p.ldb / 4 + p.N / 256 : p.ldb) >= (1L << 32)) return cdae_fail("lin16: product too large");
-    const unsigned g = (unsigned)blocks;
+    const long g = lay_out<AMC, BMC>(p, pl.bm, pl.splits, ws);
+    if (g < 0) return -1;
     if (pl.bm == 256 ? launch_tiles<T, AMC, BMC, 256, 2, 4, 2>(p, g, st)
         : pl.bm == 64 ? launch_tiles<T, AMC, BMC, 64, 4, 1, 4>(p, g, st)
         : pl.slots == 4 ? launch_tiles<T, AMC, BMC, 128, 2, 2, 4>(p, g, st)
                         : launch_tiles<T, AMC, BMC, 128, 2, 2, 2>(p, g, st))
         return -1;
-    if (p.splits > 1) {
-        const long f = ((long)p.M * ((p.N + 3) / 4) + 255) / 256;
-        hipLaunchKernelGGL((lin_finish_kernel<T>), dim3((unsigned)(f < 16384 ? f : 16384)), dim3(256), 0, st, p);
-        if (hipGetLastError() != hipSuccess) return cdae_fail("lin16: launch failed");
-    }
-    return 0;
+    return finish<T>(p, st);
+}
+// px: dx [M][K] over N;  pw: dw [N][K] over M
+template <class T>
+int products(LinArgs px, LinArgs pw, char* ws, hipStream_t st) {
+    const Pair pl = pair_plan(px.M, px.K, px.N);
+    if (!pl.together) return product<T, false, true>(px, ws, st) || product<T, true, true>(pw, ws, st) ? -1 : 0;
+    const long gx = lay_out<false, true>(px, pl.bm, pl.sx, ws), gw = lay_out<true, true>(pw, pl.bm, pl.sw, ws + slab_of(px.M, px.N, pl.sx));
+    if (gx < 0 || gw < 0) return -1;
+    if (pl.bm == 256 ? launch_pair<T, 256, 2, 4, 2>(pw, px, gw, gx, st)
+        : pl.bm == 64 ? launch_pair<T, 64, 4, 1, 4>(pw, px, gw, gx, st)
+        : pl.slots == 4 ? launch_pair<T, 128, 2, 2, 4>(pw, px, gw, gx, st)
+                        : launch_pair<T, 128, 2, 2, 2>(pw, px, gw, gx, st))
+        return -1;
+    return finish<T>(px, st) || finish<T>(pw, st) ? -1 : 0;
 }
 
 int bad_dims(int M, int N, int K, int dt) {
@@ -611,11 +694,10 @@ extern "C" {
 size_t cdae_lin16_workspace_bytes(int op, int M, int N, int K) {
     if (M <= 0 || N <= 0 || K <= 0) return 0;
     const size_t x = up256((size_t)M * up8(K) * 2), w = up256((size_t)N * up8(K) * 2), d = up256((size_t)M * up8(N) * 2);
-    if (op == CDAE_LIN16_FWD) return x + w + gemm_ws(M, N, K) + 256;
+    if (op == CDAE_LIN16_FWD) return x + w + slab_of(M, N, plan(M, N, K).splits) + 256;
     if (op == CDAE_LIN16_BWD) {
         const int rows = slope_rows(M, N);
-        const size_t sums = up256(sizeof(float) * (size_t)N * ((M + rows - 1) / rows)), one = gemm_ws(M, K, N), two = gemm_ws(N, K, M);
-        const size_t most = w + x + (one > two ? one : two);
+        const size_t sums = up256(sizeof(float) * (size_t)N * ((M + rows - 1) / rows)), most = w + x + bwd_ws(M, N, K);
         return d + (sums > most ? sums : most) + 256;
     }
     return 0;
@@ -670,6 +752,7 @@ int cdae_lin16_bwd(const void* dy, long lddy, const void* x, long ldx, const voi
     pw.M = N; pw.N = K; pw.K = M; pw.y = (u16*)dw; pw.ldy = lddw;
     const Operand ow{&px.B, &px.ldb, N, K}, ox{&pw.B, &pw.ldb, M, K};
     if (dx && dw ? prepare({ow, ox}, at, st) : dx ? prepare({ow}, at, st) : dw ? prepare({ox}, at, st) : 0) return -1;
+    if (dx && dw) return dt == DT_BF16 ? products<Bf16>(px, pw, at, st) : products<F16>(px, pw, at, st);
     if (dx && (dt == DT_BF16 ? product<Bf16, false, true>(px, at, st) : product<F16, false, true>(px, at, st))) return -1;
     if (dw && (dt == DT_BF16 ? product<Bf16, true, true>(pw, at, st) : product<F16, true, true>(pw, at, st))) return -1;
     return 0;

@@ -9,6 +9,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <cmath>
@@ -71,6 +72,20 @@ bool wanted(std::initializer_list<Tensor> ts) {
     for (const Tensor& t : ts) if (t.defined() && t.requires_grad()) return true;
     return false;
 }
+// A leaf's gradient is summed on the stream on which its first live graph was made.  If that is the default stream and this forward is being captured, the
+// captured backward would have the default stream wait on the capture, which HIP does not allow, and the error surfaces on autograd's thread, where it
+// ends the process: refused here, before anything is launched.
+void capturable(const char* who, const Tensor& x, std::initializer_list<Tensor> leaves) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing((hipStream_t)stream_of(x), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+    for (const Tensor& t : leaves) {
+        if (!t.defined() || !t.requires_grad() || !t.is_leaf()) continue;
+        const auto sum = torch::autograd::impl::try_get_grad_accumulator(t);
+        if (!sum) continue;
+        const std::optional<c10::Stream> on = sum->stream();
+        REFUSE(!on || on->id() != 0, who, ": captured while an eager graph over the same leaf, made on the default stream, is alive; free its results first");
+    }
+}
 // first derivatives only: with create_graph the gradients lead to a node that says so
 variable_list once(variable_list&& g) {
     if (!at::GradMode::is_enabled()) return std::move(g);
@@ -90,6 +105,13 @@ int act_of(const std::string& a) {
     throw Refused("linear_act: act is one of none, silu, relu, gelu, gelu_tanh");
 }
 
+bool as_it_lies(const Rows& r) {
+    return r.t.size(-1) % 8 == 0 && r.pitch % 8 == 0 && r.pitch <= 1L << 22 && reinterpret_cast<uintptr_t>(r.t.const_data_ptr()) % 16 == 0;
+}
+size_t linear_scratch(int op, const Rows& x, const Rows& w, int64_t M) {
+    return cdae_lin16_workspace_bytes(op | (as_it_lies(x) && as_it_lies(w) ? CDAE_LIN16_ALIGNED : 0), (int)M, (int)w.t.size(0), (int)w.t.size(1));
+}
+
 Tensor linear_forward(const Rows& x, const Rows& w, const Tensor& b, const Tensor& res_, int act, Tensor* z, const Tensor& x_as_given) {
     const int64_t K = w.t.size(1), N = w.t.size(0), M = x.t.numel() / K;
     std::vector<int64_t> shape(x_as_given.sizes().begin(), x_as_given.sizes().end());
@@ -99,7 +121,7 @@ Tensor linear_forward(const Rows& x, const Rows& w, const Tensor& b, const Tenso
     if (!M) return y;
     const Tensor bias = b.defined() ? b.contiguous() : b;
     const Rows res = rows_of(res_, N);
-    const size_t need = cdae_lin16_workspace_bytes(CDAE_LIN16_FWD, (int)M, (int)N, (int)K);
+    const size_t need = linear_scratch(CDAE_LIN16_FWD, x, w, M);
     const Tensor ws = scratch(need, x.t);
     check(cdae_lin16_fwd(ptr(x.t), x.pitch, ptr(w.t), w.pitch, ptr(bias), ptr(res.t), res.pitch, mptr(y), N, z ? mptr(*z) : nullptr, N, (int)M, (int)N, (int)K, act,
                          type_of(x.t), mptr(ws), need, stream_of(x.t)));
@@ -141,7 +163,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
             return once(std::move(g));
         }
         const Rows x = rows_of(xt, K), w = rows_of(wt, K), dy = rows_of(dy_, N);
-        const size_t need = cdae_lin16_workspace_bytes(CDAE_LIN16_BWD, (int)M, (int)N, (int)K);
+        const size_t need = linear_scratch(CDAE_LIN16_BWD, x, w, M);
         const Tensor ws = scratch(need, xt);
         check(cdae_lin16_bwd(ptr(dy.t), dy.pitch, ptr(x.t), x.pitch, ptr(w.t), w.pitch, ptr(z), N, mptr(g[0]), K, mptr(g[1]), K, mptr(g[2]), (int)M, (int)N, (int)K,
                              (int)ctx->saved_data["act"].toInt(), type_of(xt), mptr(ws), need, stream_of(xt)));
@@ -165,9 +187,12 @@ Tensor linear_act(const Tensor& x, const Tensor& w, const std::optional<Tensor>&
         for (int64_t i = 0; ok && i + 1 < x.dim(); ++i) ok = res.size(i) == x.size(i);
         REFUSE(ok, "linear_act: a residual of the result's shape (nothing is broadcast)");
     }
-    REFUSE(x.numel() / K <= (1LL << 30) && N <= (1LL << 24) && K <= (1LL << 24), "linear_act: at most 2^30 rows and 2^24 features");
+    REFUSE(x.numel() / K <= (1LL << 30) && N <= (1LL << 22) && K <= (1LL << 22), "linear_act: at most 2^30 rows and 2^22 features");
     c10::DeviceGuard on(x.device());
-    if (wanted({x, w, b, res})) return LinearAct::apply(x, w, maybe(b), maybe(res), (int64_t)act);
+    if (wanted({x, w, b, res})) {
+        capturable("linear_act", x, {x, w, b, res});
+        return LinearAct::apply(x, w, maybe(b), maybe(res), (int64_t)act);
+    }
     return linear_forward(rows_of(x, K), rows_of(w, K), b, res, act, nullptr, x);
 }
 
@@ -321,6 +346,7 @@ py::tuple residual_norm(const Tensor& x, const std::optional<Tensor>& f_, const 
     c10::DeviceGuard on(x.device());
     variable_list out;
     if (wanted({x, f, vec[0], vec[1], vec[2], w[0], w[1], w[2], w[3]})) {
+        capturable(who, x, {x, f, vec[0], vec[1], vec[2], w[0], w[1], w[2], w[3]});
         out = ResidualNorm::apply(x, maybe(f), maybe(vec[0]), maybe(vec[1]), maybe(vec[2]), maybe(w[0]), maybe(w[1]), maybe(w[2]), maybe(w[3]), c);
     } else {
         Tensor t[T_COUNT] = {x, f, vec[0], vec[1], vec[2], w[0], w[1], w[2], w[3]};

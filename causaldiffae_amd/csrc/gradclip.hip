@@ -282,7 +282,7 @@ size_t cdae_grad_workspace_bytes(void) { return sizeof(double) * GC_SLOTS; }
 int cdae_grad_norm(const void* const* in, const long* n, const int* types, int count, double scale, double max_norm, float* norm, void* ws, size_t ws_bytes,
                    void* stream) {
     if (check_list("grad_norm: a list of device tensors with sizes >= 0 and types 0 (bf16), 1 (fp16), 2 (fp32)", in, n, types, count)) return -1;
-    if (!norm || !ws || ws_bytes < cdae_grad_workspace_bytes()) return cdae_fail("grad_norm: norm[2] and a workspace of cdae_grad_workspace_bytes() required");
+    if (!norm || !ws || ((size_t)ws & 15) || ws_bytes < cdae_grad_workspace_bytes()) return cdae_fail("grad_norm: norm[2] and a workspace of cdae_grad_workspace_bytes() required");
     if (!(max_norm >= 0.0)) return cdae_fail("grad_norm: max_norm must be a number >= 0 (infinity: nothing is clipped)");
     hipStream_t st = (hipStream_t)stream;
     const double bytes = bytes_in(n, types, count);
@@ -298,7 +298,7 @@ int cdae_grad_clip(const void* const* in, const long* n, const int* types, void*
                    float* norm, void* ws, size_t ws_bytes, void* stream) {
     if (check_list("grad_clip: a list of device tensors with sizes >= 0 and types 0 (bf16), 1 (fp16), 2 (fp32)", in, n, types, count)) return -1;
     if (check_list("grad_clip: outputs beside every input, types 0 (bf16), 1 (fp16), 2 (fp32)", (const void* const*)out, n, out_types, count)) return -1;
-    if (!norm || !ws || ws_bytes < cdae_grad_workspace_bytes()) return cdae_fail("grad_clip: norm[2] and a workspace of cdae_grad_workspace_bytes() required");
+    if (!norm || !ws || ((size_t)ws & 15) || ws_bytes < cdae_grad_workspace_bytes()) return cdae_fail("grad_clip: norm[2] and a workspace of cdae_grad_workspace_bytes() required");
     if (!(max_norm >= 0.0)) return cdae_fail("grad_clip: max_norm must be a number >= 0 (infinity: nothing is clipped)");
     if (const int rc = check_overlap(in, n, types, out, out_types, count))
         return cdae_fail(rc == 1 ? "grad_clip: two outputs share memory, or an output shares memory with a gradient other than its own" : "grad_clip: out of host memory");

@@ -563,14 +563,16 @@ size_t bwd_ws(int M, int N, int K) {
     return one > both ? one : both;                                       // (a call may want one product only)
 }
 
-// Operands in the form the tile kernel reads: 16-byte pieces, rows of a multiple of 8 values.  Those that are not are copied into `ws` by one launch.
+// Operands in the form the tile kernel reads: 16-byte pieces, rows of a multiple of 8 values, at most 2^22 from row to row (a lane's offsets inside a
+// stage are 32 bits).  Those that are not are copied into `ws` by one launch.
+bool as_it_lies(const void* X, long ldx, int cols) { return cols % 8 == 0 && ldx % 8 == 0 && ldx <= 1L << 22 && al16(X); }
 struct Operand { const u16** X; long* ldx; long rows; int cols; };
 int prepare(std::initializer_list<Operand> ops, char*& ws, hipStream_t st) {
     PadJobs jobs{};
     int n = 0;
     long most = 0;
     for (const Operand& o : ops) {
-        if (o.cols % 8 == 0 && *o.ldx % 8 == 0 && al16(*o.X)) continue;
+        if (as_it_lies(*o.X, *o.ldx, o.cols)) continue;
         const long pitch = up8(o.cols), pieces = o.rows * (pitch / 8);
         u16* dst = (u16*)ws;
         ws += up256((size_t)o.rows * pitch * 2);
@@ -666,7 +668,7 @@ int products(LinArgs px, LinArgs pw, char* ws, hipStream_t st) {
 
 int bad_dims(int M, int N, int K, int dt) {
     if (M < 0 || N <= 0 || K <= 0) return cdae_fail("lin16: M >= 0, N >= 1 and K >= 1 required");
-    if (M > 1 << 30 || N > 1 << 24 || K > 1 << 24) return cdae_fail("lin16: at most 2^30 rows and 2^24 features");
+    if (M > 1 << 30 || N > 1 << 22 || K > 1 << 22) return cdae_fail("lin16: at most 2^30 rows and 2^22 features");
     if (dt != DT_BF16 && dt != DT_F16) return cdae_fail("lin16: type 0 (bf16) or 1 (fp16)");
     return 0;
 }
@@ -693,14 +695,17 @@ extern "C" {
 
 size_t cdae_lin16_workspace_bytes(int op, int M, int N, int K) {
     if (M <= 0 || N <= 0 || K <= 0) return 0;
-    const size_t x = up256((size_t)M * up8(K) * 2), w = up256((size_t)N * up8(K) * 2), d = up256((size_t)M * up8(N) * 2);
-    if (op == CDAE_LIN16_FWD) return x + w + slab_of(M, N, plan(M, N, K).splits) + 256;
-    if (op == CDAE_LIN16_BWD) {
-        const int rows = slope_rows(M, N);
-        const size_t sums = up256(sizeof(float) * (size_t)N * ((M + rows - 1) / rows)), most = w + x + bwd_ws(M, N, K);
-        return d + (sums > most ? sums : most) + 256;
+    const bool copies = !(op & CDAE_LIN16_ALIGNED);
+    const size_t x = copies ? up256((size_t)M * up8(K) * 2) : 0, w = copies ? up256((size_t)N * up8(K) * 2) : 0;
+    switch (op & ~CDAE_LIN16_ALIGNED) {
+        case CDAE_LIN16_FWD: return x + w + slab_of(M, N, plan(M, N, K).splits) + 256;
+        case CDAE_LIN16_BWD: {
+            const int rows = slope_rows(M, N);
+            const size_t sums = up256(sizeof(float) * (size_t)N * ((M + rows - 1) / rows)), most = w + x + bwd_ws(M, N, K);
+            return up256((size_t)M * up8(N) * 2) + (sums > most ? sums : most) + 256;
+        }
+        default: return 0;
     }
-    return 0;
 }
 
 int cdae_lin16_fwd(const void* x, long ldx, const void* w, long ldw, const void* bias, const void* res, long ldres, void* y, long ldy, void* z, long ldz, int M,
@@ -709,7 +714,8 @@ int cdae_lin16_fwd(const void* x, long ldx, const void* w, long ldw, const void*
     if (!known_act(act)) return cdae_fail("lin16_fwd: activation 0 (none), 1 (SiLU), 3 (ReLU), 5 (GELU) or 6 (GELU, tanh form)");
     if (M == 0) return 0;
     if (!x || !w || !y || ldx < K || ldw < K || ldy < N || (res && ldres < N) || (z && ldz < N)) return cdae_fail("lin16_fwd: x, w, y and row pitches of at least a row required");
-    if (ws_bytes < cdae_lin16_workspace_bytes(CDAE_LIN16_FWD, M, N, K) || !ws) return cdae_fail("lin16_fwd: workspace of cdae_lin16_workspace_bytes() required");
+    const int lies = as_it_lies(x, ldx, K) && as_it_lies(w, ldw, K) ? CDAE_LIN16_ALIGNED : 0;
+    if (!ws || !al16(ws) || ws_bytes < cdae_lin16_workspace_bytes(CDAE_LIN16_FWD | lies, M, N, K)) return cdae_fail("lin16_fwd: workspace of cdae_lin16_workspace_bytes() required");
     hipStream_t st = (hipStream_t)stream;
     const Timed timed(PROF_IGEMM, 2.0 * M * N * K, 2.0 * ((double)M * K + (double)N * K + (double)M * N * (1 + (res != nullptr) + (z != nullptr))), st);
     LinArgs p{};
@@ -728,12 +734,13 @@ int cdae_lin16_bwd(const void* dy, long lddy, const void* x, long ldx, const voi
     if (M == 0) return cdae_fail("lin16_bwd: no rows");
     if (!dy || lddy < N || (act != L_NONE && (!z || ldz < N))) return cdae_fail("lin16_bwd: dy, and z with an activation, required");
     if ((dx && (!w || ldw < K || lddx < K)) || (dw && (!x || ldx < K || lddw < K))) return cdae_fail("lin16_bwd: w for dx, x for dw, row pitches of at least a row");
-    if (!ws || ws_bytes < cdae_lin16_workspace_bytes(CDAE_LIN16_BWD, M, N, K)) return cdae_fail("lin16_bwd: workspace of cdae_lin16_workspace_bytes() required");
+    const int lies = (!dx || as_it_lies(w, ldw, K)) && (!dw || as_it_lies(x, ldx, K)) ? CDAE_LIN16_ALIGNED : 0;
+    if (!ws || !al16(ws) || ws_bytes < cdae_lin16_workspace_bytes(CDAE_LIN16_BWD | lies, M, N, K)) return cdae_fail("lin16_bwd: workspace of cdae_lin16_workspace_bytes() required");
     hipStream_t st = (hipStream_t)stream;
     const Timed timed(PROF_IGEMM, 2.0 * M * N * K * ((dx != nullptr) + (dw != nullptr)),
                       2.0 * ((double)M * N * (act ? 2 : 1) + (double)M * K * ((dx != nullptr) + (dw != nullptr)) + (double)N * K * ((dx != nullptr) + (dw != nullptr))), st);
     char* at = (char*)ws;
-    const bool copy = act != L_NONE || N % 8 || lddy % 8 || !al16(dy);
+    const bool copy = act != L_NONE || !as_it_lies(dy, lddy, N);
     u16* dz = nullptr;
     if (copy && (dx || dw)) { dz = (u16*)at; at += up256((size_t)M * up8(N) * 2); }
     if (dz || dbias) {

@@ -566,7 +566,7 @@ int cdae_resnorm_bwd(const cdae_resnorm* p, void* stream) {
     if ((p->dgate && !p->gate) || (p->dscale && !p->scale) || (p->dshift && !p->shift) || (p->dw1 && !p->w1) || (p->db1 && !p->b1) || (p->dw2 && !p->w2) ||
         (p->db2 && !p->b2))
         return cdae_fail("resnorm_bwd: a gradient of a vector that is not there");
-    if (!p->ws || p->ws_bytes < cdae_resnorm_workspace_bytes(p->B, p->T, p->C)) return cdae_fail("resnorm_bwd: workspace of cdae_resnorm_workspace_bytes() required");
+    if (!p->ws || ((size_t)p->ws & 15) || p->ws_bytes < cdae_resnorm_workspace_bytes(p->B, p->T, p->C)) return cdae_fail("resnorm_bwd: workspace of cdae_resnorm_workspace_bytes() required");
     hipStream_t st = (hipStream_t)stream;
     const double rows = (double)p->B * p->T * p->C * (p->dt == DT_F32 ? 4 : 2) * (1 + (p->f != nullptr) + (p->dr != nullptr) + (p->du != nullptr) + (p->dx != nullptr) + (p->df != nullptr));
     const Timed timed(PROF_GN, rows, rows, st);

@@ -10,9 +10,9 @@ Rows are the last dimension: an activation [N, C, H, W] in this package's NHWC s
 
 Sums, statistics and products accumulate in fp32 (the norm of the gradients in fp64) and every result is rounded once.  Calls run on the current
 stream of their tensors' device, allocate their scratch themselves for the one call, neither synchronise nor copy to the host, keep nothing between
-calls and can be captured into a graph.  (As with every differentiable operator, a backward pass is captured only while no eager graph over the same
-leaves is alive.)  Gradients are first derivatives; a second one raises.  Wrong arguments raise CdaeError; there is no CPU form.  The checks and the
-autograd nodes are native (csrc/block_ext.cpp): the kernels of a call are shorter than the same dispatch from Python.
+calls and can be captured into a graph.  (A backward pass can be captured only while no eager graph over the same leaves, made on the default stream,
+is alive: the captured forward raises then.)  Gradients are first derivatives; a second one raises.  Wrong tensors and values raise CdaeError; there is
+no CPU form.  The checks and the autograd nodes are native (csrc/block_ext.cpp): the kernels of a call are shorter than the same dispatch from Python.
 """
 import torch
 
@@ -31,7 +31,7 @@ MAX_FEATURES = 8192          # widest row of residual_norm
 def linear_act(x, w, b=None, res=None, act="none"):
     """y = act(x @ w^T + b) + res for rows x [..., K], a weight [N, K], a bias [N] and a residual [..., N], all bf16 or all fp16; y has their type.
     act: "none", "silu", "relu", "gelu" or "gelu_tanh".  Where a gradient is wanted the pre-activation is kept in fp16 beside x and w.  Rows at any
-    pitch and alignment are taken as they are; fp32 rows belong to ops.linear."""
+    pitch and alignment are taken; fp32 rows belong to ops.linear."""
     return _ext.linear_act(x, w, b, res, act)
 
 

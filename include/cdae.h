@@ -574,13 +574,16 @@ int cdae_wprep_all_m16(const float* flat, const void* desc, int nw, int total_ti
                        unsigned short* kb_lo, const float* w_scales, void* stream);
 
 /* ---- a feed-forward block on rows: linear layers with an activation, the norms around the block, and the step that trains it.
-   Row types: 0 bf16, 1 fp16, 2 fp32 (the linear layers: 0 or 1).  Nothing is kept between calls; workspaces belong to one call at a time. */
+   Row types: 0 bf16, 1 fp16, 2 fp32 (the linear layers: 0 or 1).  Nothing is kept between calls; workspaces are 16-byte aligned and belong to
+   one call at a time. */
 /* y[M][N] = act(x[M][K] @ w[N][K]^T + bias) + res on 16-bit rows, fp32 accumulation, one rounding (lin16.hip).  Operands of one 16-bit type at any
    pitch >= a row and any alignment; bias [N] and res [M][N] may be NULL.  act: 0 none, 1 SiLU, 3 ReLU, 5 GELU, 6 GELU in its tanh form.  z (may be
    NULL; for the backward) receives the pre-activation as fp16 whatever dt is (beyond fp16's range: infinity, whose slope is taken at the range's end).
    cdae_lin16_bwd: dx = dz @ w, dw = dz^T @ x, dbias = column sums of dz with dz = dy * act'(z) (rounded to the rows' type as an operand of the
    products; the sums take it unrounded); each result may be NULL.  The gradient of res is dy itself. */
-enum { CDAE_LIN16_FWD = 0, CDAE_LIN16_BWD = 1 };
+/* workspace: with CDAE_LIN16_ALIGNED added to the operation x and w are 16-byte aligned, K is a multiple of 8 and so are their pitches, which are
+   at most 2^22: room for their copies is not counted (a call asks for what its own operands need) */
+enum { CDAE_LIN16_FWD = 0, CDAE_LIN16_BWD = 1, CDAE_LIN16_ALIGNED = 8 };
 size_t cdae_lin16_workspace_bytes(int op, int M, int N, int K);
 int cdae_lin16_fwd(const void* x, long ldx, const void* w, long ldw, const void* bias, const void* res, long ldres, void* y, long ldy, void* z, long ldz, int M,
                    int N, int K, int act, int dt, void* ws, size_t ws_bytes, void* stream);

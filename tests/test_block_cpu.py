@@ -20,6 +20,9 @@ def test_workspace_sizes():
     for op in (0, 1):
         assert lib.cdae_lin16_workspace_bytes(op, 1, 1, 1) > 0
         assert lib.cdae_lin16_workspace_bytes(op, 1 << 20, 4096, 4096) >= (1 << 20) * 4096 * 2         # (sizes beyond 32 bits)
+        copies = ((1 << 20) + 4096) * 4096 * 2                                                         # (of operands that the kernel cannot read as they lie)
+        spared = lib.cdae_lin16_workspace_bytes(op, 1 << 20, 4096, 4096) - lib.cdae_lin16_workspace_bytes(op | 8, 1 << 20, 4096, 4096)
+        assert copies - (1 << 24) <= spared <= copies                                                  # (the backward's partial sums share their place)
     assert lib.cdae_resnorm_workspace_bytes(1, 1, 8193) == 0 and lib.cdae_resnorm_workspace_bytes(0, 1, 8) == 0
     assert lib.cdae_resnorm_workspace_bytes(1, 1, 8192) >= 4 * 4 * 8192
     assert lib.cdae_grad_workspace_bytes() >= 8 * 1024
@@ -35,7 +38,7 @@ def test_linear_refusals():
     for kw in (dict(M=-1), dict(N=0), dict(K=0)):
         refused(fwd(**kw), "required")
         refused(bwd(**kw), "required")
-    for kw in (dict(M=(1 << 30) + 1), dict(N=(1 << 24) + 1), dict(K=(1 << 24) + 1)):
+    for kw in (dict(M=(1 << 30) + 1), dict(N=(1 << 22) + 1), dict(K=(1 << 22) + 1)):
         refused(fwd(**kw), "at most")
         refused(bwd(**kw), "at most")
     refused(fwd(dt=2), "type")
@@ -47,6 +50,8 @@ def test_linear_refusals():
         refused(fwd(**kw), "pitches")
     refused(fwd(ws_bytes=16), "workspace")
     refused(fwd(ws=None), "workspace")
+    refused(fwd(ws=PTR + 8), "workspace")
+    refused(fwd(x=PTR + 2, ws_bytes=lib.cdae_lin16_workspace_bytes(8, 4, 8, 8)), "workspace")
     refused(bwd(ws_bytes=16), "workspace")
     refused(bwd(M=0), "no rows")
     refused(bwd(dy=None), "dy")

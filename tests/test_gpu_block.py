@@ -678,6 +678,53 @@ def test_block_in_two_graphs():
             assert all(torch.equal(p, q) for p, q in zip(w, o)), k
 
 
+def test_capture_beside_an_eager_graph():
+    """a leaf whose live eager graph was made on the default stream: the captured forward is refused before it launches anything, and the capture ends
+    as any other; once that graph is gone the same step is captured"""
+    from causaldiffae_amd import CdaeError
+    x, w = rnd(1, 6, 64, dtype=BF16).requires_grad_(), rnd(2, 48, 64, dtype=BF16).requires_grad_()
+    v = rnd(3, 64).requires_grad_()
+    eager = [blk().linear_act(x, w, act="gelu"), blk().residual_norm(x.detach(), pre=v)[1]]
+    calls = [lambda: blk().linear_act(x.detach(), w, act="gelu"), lambda: blk().residual_norm(x.detach(), pre=v)[1]]
+    for call in calls:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            other = w.detach() * 2
+            with pytest.raises(CdaeError, match="alive"):
+                call()
+            with torch.no_grad():
+                call()
+        g.replay()
+        assert torch.equal(other, w.detach() * 2)
+    dy = [rnd(4 + i, *e.shape, dtype=BF16) for i, e in enumerate(eager)]
+    want = [torch.autograd.grad(e, leaf, d)[0] for e, leaf, d in zip(eager, (w, v), dy)]
+    del eager
+    torch.cuda.synchronize()
+    for call, leaf, d, one in zip(calls, (w, v), dy, want):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got, = torch.autograd.grad(call(), leaf, d)
+        for _ in range(3):
+            got.zero_()
+            g.replay()
+            assert torch.equal(got, one)
+
+
+def test_linear_act_far_rows():
+    """rows more than 2^22 values apart, forward and backward"""
+    far = (1 << 23) + 8
+    big = torch.zeros(5 * far, dtype=BF16, device=DEV)
+    away = lambda r, C: big.as_strided((5, C), (far, 1), 4096 * r)
+    x, w, dy = rnd(1, 5, 64, dtype=BF16), rnd(2, 48, 64, dtype=BF16), rnd(3, 5, 48, dtype=BF16)
+    xs, ws, ds = away(0, 64).copy_(x).requires_grad_(), w.clone().requires_grad_(), away(1, 48).copy_(dy)
+    for act in ("none", "silu"):
+        a, b = x.clone().requires_grad_(), w.clone().requires_grad_()
+        ya, yb = blk().linear_act(a, b, act=act), blk().linear_act(xs, ws, act=act)
+        assert torch.equal(ya, yb)
+        for p, q in zip(torch.autograd.grad(ya, (a, b), dy), torch.autograd.grad(yb, (xs, ws), ds)):
+            assert torch.equal(p, q)
+
+
 # ----------------------------------------------------------------------------- clipping inside the optimizer step
 def test_optimizer_step_clips():
     """FusedAdamWEMA.step(max_norm) is the step whose grad_scale is the factor of the definition, and leaves the gradients as they are"""

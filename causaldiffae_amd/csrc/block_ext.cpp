@@ -76,8 +76,9 @@ bool wanted(std::initializer_list<Tensor> ts) {
 // captured backward would have the default stream wait on the capture, which HIP does not allow, and the error surfaces on autograd's thread, where it
 // ends the process: refused here, before anything is launched.
 void capturable(const char* who, const Tensor& x, std::initializer_list<Tensor> leaves) {
+    const hipStream_t st = (hipStream_t)stream_of(x);
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing((hipStream_t)stream_of(x), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+    if (!st || hipStreamIsCapturing(st, &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;        // (the default stream is never captured)
     for (const Tensor& t : leaves) {
         if (!t.defined() || !t.requires_grad() || !t.is_leaf()) continue;
         const auto sum = torch::autograd::impl::try_get_grad_accumulator(t);
@@ -346,6 +347,7 @@ py::tuple residual_norm(const Tensor& x, const std::optional<Tensor>& f_, const 
     c10::DeviceGuard on(x.device());
     variable_list out;
     if (wanted({x, f, vec[0], vec[1], vec[2], w[0], w[1], w[2], w[3]})) {
+        REFUSE(B < (1LL << 22), who, ": with gradients fewer than 2^22 samples");
         capturable(who, x, {x, f, vec[0], vec[1], vec[2], w[0], w[1], w[2], w[3]});
         out = ResidualNorm::apply(x, maybe(f), maybe(vec[0]), maybe(vec[1]), maybe(vec[2]), maybe(w[0]), maybe(w[1]), maybe(w[2]), maybe(w[3]), c);
     } else {

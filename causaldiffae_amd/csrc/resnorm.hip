@@ -23,7 +23,7 @@
 //   * the next row is requested before this one is worked on, and the vectors are folded to four (forward) or three (backward) per chunk of rows:
 //     r = x + n1 (g w1) + g b1,   u = n2 (w2 (1 + s)) + (b2 (1 + s) + t);
 //   * sums inside a wave on the lane-permute instructions (no LDS), across waves through LDS with ONE barrier: a wave hands over (mean, sum of
-//     squares about it), which combine exactly, so a layer norm needs no second round and no difference of large sums.
+//     squares about it), of which every lane then takes one wave's and the same permutes add them up; they combine exactly, so a layer norm needs no second round and no difference of large sums.
 // All arithmetic and all sums are fp32; a result is rounded once, when it is written.
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -87,11 +87,7 @@ struct RowSum {
                 for (int i = 0; i < NV; ++i) b[(threadIdx.x >> 6) * 2 + i] = a[i];
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                a[i] = 0.f;
-#pragma unroll
-                for (int w = 0; w < W; ++w) a[i] += b[w * 2 + i];
-            }
+            for (int i = 0; i < NV; ++i) a[i] = lane_sum<W>(b[(threadIdx.x & (W - 1)) * 2 + i]);
         }
     }
     // n = the normalised row, -> 1 / sqrt(mean square + eps)
@@ -121,13 +117,11 @@ struct RowSum {
                 float* b = sh + (turn ^= 1) * (2 * W);
                 if ((threadIdx.x & 63) == 0) { b[wave * 2] = mw; b[wave * 2 + 1] = q[0]; }
                 __syncthreads();
-                float sum = 0.f;
-#pragma unroll
-                for (int w = 0; w < W; ++w) sum = fmaf(count(w), b[2 * w], sum);
-                m = sum * inv_c;
-                q[0] = 0.f;
-#pragma unroll
-                for (int w = 0; w < W; ++w) { const float d = b[2 * w] - m; q[0] += fmaf(count(w) * d, d, b[2 * w + 1]); }
+                const int w = threadIdx.x & (W - 1);
+                const float its = count(w), itsm = b[2 * w];
+                m = lane_sum<W>(its * itsm) * inv_c;
+                const float d = itsm - m;
+                q[0] = lane_sum<W>(fmaf(its * d, d, b[2 * w + 1]));
             }
         }
         const float i = 1.f / sqrtf(q[0] * inv_c + eps);
@@ -281,6 +275,10 @@ __global__ __launch_bounds__(block_of(TPR)) void rn_bwd_kernel(const RnArgs a) {
     constexpr int BLOCK = block_of(TPR), GROUPS = BLOCK / TPR;
     __shared__ float sh[TPR > 64 ? 4 * (TPR / 64) : 1];
     __shared__ float cols[GROUPS > 1 ? GROUPS * TPR * RN_V : 1];
+    // rows of 1024 threads: a thread has 128 registers, and its three vectors (24) lie in LDS, each thread its own (2 x 1024 rows of 8192 bf16: 62 us;
+    // with the vectors in registers and scratch 74)
+    constexpr bool IN_LDS = TPR == 1024;
+    __shared__ float4 vecs[IN_LDS ? 6 * TPR : 1];
     const cdae_resnorm& p = a.p;
     const int lane = threadIdx.x & (TPR - 1), grp = threadIdx.x / TPR;
     const Cols<SMALL> k(lane, p.C);
@@ -302,10 +300,25 @@ __global__ __launch_bounds__(block_of(TPR)) void rn_bwd_kernel(const RnArgs a) {
     const long lf = F ? p.ld_f : p.ld_x, lr = R ? p.ld_dr : p.ld_x, lu = U ? p.ld_du : p.ld_x;
     auto row_of = [&](int t) { return t + grp < t1 ? t + grp : t1 - 1; };
     int t = row_of(t0);
-    constexpr bool AHEAD = TPR < 1024;                            // (1024 threads have 128 registers each: none left for the next row)
+    constexpr bool AHEAD = TPR < 1024 || sizeof(T) == 2;          // (1024 threads of fp32 rows have no registers left for the next row: 115 us, with it 128)
     Pack<T, RN_V> xr = k.raw(X + t * p.ld_x), fr = k.raw(Fs + t * lf), rr = k.raw(Rs + t * lr), ur = k.raw(Us + t * lu);
     float gw[RN_V], gb[RN_V], sw[RN_V], sb[RN_V];
     fold_cols<T, SMALL>(p, b, k, gw, gb, sw, sb);
+    if constexpr (IN_LDS)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            vecs[h * TPR + lane] = {gw[4 * h], gw[4 * h + 1], gw[4 * h + 2], gw[4 * h + 3]};
+            vecs[(2 + h) * TPR + lane] = {gb[4 * h], gb[4 * h + 1], gb[4 * h + 2], gb[4 * h + 3]};
+            vecs[(4 + h) * TPR + lane] = {sw[4 * h], sw[4 * h + 1], sw[4 * h + 2], sw[4 * h + 3]};
+        }
+    auto again = [&](int j, float (&v)[RN_V]) {
+        if constexpr (IN_LDS)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float4 q = vecs[(2 * j + h) * TPR + lane];
+                v[4 * h] = q.x; v[4 * h + 1] = q.y; v[4 * h + 2] = q.z; v[4 * h + 3] = q.w;
+            }
+    };
     float A[4][RN_V];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -333,12 +346,15 @@ __global__ __launch_bounds__(block_of(TPR)) void rn_bwd_kernel(const RnArgs a) {
                 for (int e = 0; e < RN_V; ++e) f[e] = n1[e];
                 i1 = rows.normalise(f, n1, k.skip, k.end, p.C, p.layer, inv_c, p.eps);
             }
+            again(0, gw);
+            again(1, gb);
 #pragma unroll
             for (int e = 0; e < RN_V; ++e) r[e] = fmaf(n1[e], gw[e], r[e]) + gb[e];
         }
         if (U) {
             const float i2 = rows.normalise(r, n2, k.skip, k.end, p.C, p.layer, inv_c, p.eps);
             float s[2] = {0.f, 0.f};
+            again(2, sw);
 #pragma unroll
             for (int e = 0; e < RN_V; ++e) {
                 A[2][e] = fmaf(live * h[e], n2[e], A[2][e]);
@@ -354,6 +370,7 @@ __global__ __launch_bounds__(block_of(TPR)) void rn_bwd_kernel(const RnArgs a) {
         if (p.dx) k.put(reinterpret_cast<T*>(p.dx) + out + (long)t * p.C, D);
         if (F) {
             float s[2] = {0.f, 0.f};
+            again(0, gw);
 #pragma unroll
             for (int e = 0; e < RN_V; ++e) {
                 A[0][e] = fmaf(live * D[e], n1[e], A[0][e]);
@@ -465,20 +482,23 @@ int threads_per_row(int C) {
     return t < 8 ? 8 : t;
 }
 
-// Backward: chunks of a sample for about 512 blocks in all, a multiple of the block's groups of rows each: two a CU (256 where a row takes 512 threads and
-// more), so that all run at once at the 140 registers a thread takes and leave few partial sums (8 x 4096 rows of 2048 bf16: 177 us; 256 blocks 234, 1024
-// blocks 202; 4 x 2048 rows of 4096: 108 us; 256 blocks 100).  Forward: a group's chunk,
-// for about 16 waves a CU; longer chunks read the vectors less often, but past 16 rows that is nothing.
-void chunks_of(int B, int T, int C, int& nch, int& rows) {
-    const int tpr = threads_per_row(C), groups = block_of(tpr) / tpr;
-    const long want = ((tpr >= 512 ? 256 : 512) + B - 1) / B;
-    rows = (int)((T + want - 1) / want);
+// Backward: chunks of a sample, a multiple of the block's groups of rows each, for as many blocks in all as run at once at 140 to 160 registers a thread,
+// and not one more (30 x 1000 rows of 512 fp16: 53 us for 510 blocks, 61 for 540): more blocks leave more partial sums.  Two blocks of 256 threads a CU (8 x 4096
+// rows of 2048 bf16: 179 us; 256 blocks 234, 768 blocks 187), one of 512 and more (4 x 2048 rows of 4096: 100 us; two 108), and of blocks of 128 threads
+// six, or four on fp32 rows (30000 rows of 600 fp16: 93 us; 1024 blocks 100, 512 blocks 156; 11 x 1700 of 700 fp32: 81; 1536 blocks 85, 512 blocks 96).
+void chunks_of(int B, int T, int C, bool wide, int& nch, int& rows) {
+    const int tpr = threads_per_row(C), groups = block_of(tpr) / tpr, at_once = tpr >= 512 ? 256 : tpr == 128 ? (wide ? 1024 : 1536) : 512;
+    const int want = B < at_once ? at_once / B : 1;
+    rows = (T + want - 1) / want;
     rows = (rows + groups - 1) / groups * groups;
     nch = (T + rows - 1) / rows;
 }
+// Forward: a group's rows, so that the 16 waves a CU that run at once take them all (4 x 2000 rows of 4000 fp16: 58 us, and 75 where a few blocks are left
+// for a second round), up to 16 rows; where that takes more rounds, 8 rows each for an even end (8 x 4096 rows of 2048 bf16: 103 us; 16 rows 110), and 16 of
+// the widest rows (8000 rows of 8000 fp16: 116 us; 8 rows 121).
 void fwd_chunks(int B, int T, int C, int& nch, int& rows) {
-    const long tpr = threads_per_row(C), r = (long)B * T * tpr / 64 / 4096;
-    rows = r < 1 ? 1 : r > 16 ? 16 : (int)r;
+    const long tpr = threads_per_row(C), r = ((long)B * T * tpr / 64 + 4095) / 4096;
+    rows = r < 1 ? 1 : r <= 16 ? (int)r : tpr == 1024 ? 16 : 8;
     nch = (T + rows - 1) / rows;
 }
 
@@ -522,7 +542,7 @@ template <class T>
 void bwd(const cdae_resnorm* p, hipStream_t st) {
     RnArgs a;
     a.p = *p;
-    chunks_of(p->B, p->T, p->C, a.nch, a.rows_per_chunk);
+    chunks_of(p->B, p->T, p->C, sizeof(T) == 4, a.nch, a.rows_per_chunk);
     float* sums = p->ws + (long)p->B * a.nch * 4 * p->C;
 #define RN_CALL(N, S) hipLaunchKernelGGL((rn_bwd_kernel<T, N, S>), dim3((unsigned)((long)p->B * a.nch)), dim3(block_of(N)), 0, st, a)
     RN_TPR(RN_CALL)
@@ -540,9 +560,10 @@ extern "C" {
 
 size_t cdae_resnorm_workspace_bytes(int B, int T, int C) {
     if (B <= 0 || T <= 0 || C <= 0 || C > RN_MAX_C) return 0;
-    int nch, rows;
-    chunks_of(B, T, C, nch, rows);
-    return sizeof(float) * 4 * (size_t)C * B * nch + sizeof(float) * RN_SUMS * (size_t)C * B;
+    int nch, nch32, rows;
+    chunks_of(B, T, C, false, nch, rows);
+    chunks_of(B, T, C, true, nch32, rows);
+    return sizeof(float) * 4 * (size_t)C * B * (nch > nch32 ? nch : nch32) + sizeof(float) * RN_SUMS * (size_t)C * B;
 }
 
 int cdae_resnorm_fwd(const cdae_resnorm* p, void* stream) {

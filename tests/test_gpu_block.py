@@ -341,6 +341,15 @@ def test_residual_norm_sizes(B, T, C, dtype):
     check_norm(r(1), r(2), v, 0.7, post, True, kind, dr=r(3), du=r(4))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("B,T,C,kind,post", [(2, 300, 4100, "layer", True), (1, 600, 8192, "rms", True), (3, 400, 5001, "layer", False), (1, 5000, 600, "rms", True)])
+def test_residual_norm_walks(B, T, C, kind, post, dtype):
+    """several rows for every block, forward and backward"""
+    v = vectors(B, C, dtype, "sample", "sample", post, True)
+    r = lambda s: rnd(s, B, T, C, dtype=dtype)
+    check_norm(r(1), r(2), v, 0.7, post, True, kind, dr=r(3), du=r(4))
+
+
 @pytest.mark.parametrize("gate", [None, "channel", "sample"])
 @pytest.mark.parametrize("mod", [None, "channel", "sample"])
 @pytest.mark.parametrize("vec,w", [(BF16, F32), (F32, BF16)])

@@ -427,7 +427,7 @@ __global__ __launch_bounds__(256) void lin_pad_kernel(const PadJobs jobs) {
 // LAST 8 values (its neighbour's are among them, written twice with the same value and summed once).  SMALL: rows of fewer than 8 values.
 template <class T, bool SMALL>
 __global__ __launch_bounds__(256) void lin_slope_kernel(const T* __restrict__ dy, long lddy, const F16* __restrict__ z, long ldz, T* __restrict__ dz, long lddz,
-                                                        float* __restrict__ part, int M, int N, int rows_per_block, int ncb, int act) {
+                                                        float* __restrict__ part, T* __restrict__ db, int M, int N, int rows_per_block, int ncb, int act) {
     __shared__ float sh[8][256];
     const int cb = blockIdx.x % ncb, rb = blockIdx.x / ncb;
     const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
@@ -463,7 +463,7 @@ __global__ __launch_bounds__(256) void lin_slope_kernel(const T* __restrict__ dy
                 for (int e = N; e < lddz; ++e) st1(dz[r * lddz + e], 0.f);
         }
     }
-    if (!part) return;
+    if (!part && !db) return;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         const int at = c + e - cb * 256;                                   // (columns before this thread's own are its neighbour's sums too)
@@ -475,7 +475,8 @@ __global__ __launch_bounds__(256) void lin_slope_kernel(const T* __restrict__ dy
         float t = 0.f;
 #pragma unroll
         for (int r = 0; r < 8; ++r) t += sh[r][threadIdx.x];
-        part[(long)rb * N + cc] = t;
+        if (db) st1(db[cc], t);                                            // (one block of rows: its sums are the result)
+        else part[(long)rb * N + cc] = t;
     }
 }
 // the column sums of the blocks, in order: 32 columns x 32 lanes of blocks
@@ -690,8 +691,8 @@ template <class T>
 void slope_launch(const void* dy, long lddy, const void* z, long ldz, u16* dz, float* part, void* dbias, int M, int N, int act, hipStream_t st) {
     const int ncb = (N + 255) / 256, rows = slope_rows(M, N), rb = (M + rows - 1) / rows;
     auto* kernel = N < 8 ? &lin_slope_kernel<T, true> : &lin_slope_kernel<T, false>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(ncb * rb)), dim3(256), 0, st, (const T*)dy, lddy, (const F16*)z, ldz, (T*)dz, up8(N), part, M, N, rows, ncb, act);
-    if (dbias) hipLaunchKernelGGL((lin_bias_kernel<T>), dim3((N + 31) / 32), dim3(1024), 0, st, part, rb, N, (T*)dbias);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(ncb * rb)), dim3(256), 0, st, (const T*)dy, lddy, (const F16*)z, ldz, (T*)dz, up8(N), part, rb == 1 ? (T*)dbias : nullptr, M, N, rows, ncb, act);
+    if (dbias && rb > 1) hipLaunchKernelGGL((lin_bias_kernel<T>), dim3((N + 31) / 32), dim3(1024), 0, st, part, rb, N, (T*)dbias);
 }
 
 }  // namespace

@@ -72,13 +72,16 @@ bool wanted(std::initializer_list<Tensor> ts) {
     for (const Tensor& t : ts) if (t.defined() && t.requires_grad()) return true;
     return false;
 }
+bool capturing(at::Device dev) {
+    const hipStream_t st = c10::hip::getCurrentHIPStream(dev.index()).stream();
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    return st && hipStreamIsCapturing(st, &status) == hipSuccess && status != hipStreamCaptureStatusNone;      // (the default stream is never captured)
+}
 // A leaf's gradient is summed on the stream on which its first live graph was made.  If that is the default stream and this forward is being captured, the
 // captured backward would have the default stream wait on the capture, which HIP does not allow, and the error surfaces on autograd's thread, where it
 // ends the process: refused here, before anything is launched.
 void capturable(const char* who, const Tensor& x, std::initializer_list<Tensor> leaves) {
-    const hipStream_t st = (hipStream_t)stream_of(x);
-    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    if (!st || hipStreamIsCapturing(st, &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;        // (the default stream is never captured)
+    if (!capturing(x.device())) return;
     for (const Tensor& t : leaves) {
         if (!t.defined() || !t.requires_grad() || !t.is_leaf()) continue;
         const auto sum = torch::autograd::impl::try_get_grad_accumulator(t);
@@ -410,6 +413,7 @@ Tensor clip_grad_norm(const py::object& grads, double max_norm, double scale, co
     at::NoGradGuard no_grad;
     List src(who, grads);
     c10::DeviceGuard on(src.dev);
+    REFUSE(!error_if_nonfinite || !capturing(src.dev), who, ": error_if_nonfinite waits for the device and cannot be captured");
     std::vector<std::pair<Tensor, Tensor>> later;              // (tensor with gaps, dense copy): written back at the end
     List dst = out.is_none() ? src : List(who, out);
     REFUSE(dst.t.size() == src.t.size(), who, ": an output for every gradient");

@@ -75,5 +75,6 @@ def clip_grad_norm_(grads, max_norm, scale=1.0, out=None, error_if_nonfinite=Fal
     grads: the gradients themselves ([p.grad for p in model.parameters() if p.grad is not None]), any sizes and strides, bf16 / fp16 / fp32 mixed.
     scale: what the gradients have to be multiplied by first (1 / loss scale, 1 / ranks of a sum).  out: None (in place), or tensors of the same shapes
     and any of the types, e.g. fp32 master gradients; outputs may not share memory with each other or with another gradient.  A norm that is not finite
-    leaves zeros or NaN: error_if_nonfinite=True raises instead, before anything is written, at the cost of waiting for the device."""
+    leaves zeros or NaN: error_if_nonfinite=True raises instead, before anything is written, at the cost of waiting for the device
+    (and so not inside a captured graph)."""
     return _ext.clip_grad_norm_(grads, max_norm, scale, out, error_if_nonfinite)

@@ -701,6 +701,8 @@ def test_capture_beside_an_eager_graph():
             other = w.detach() * 2
             with pytest.raises(CdaeError, match="alive"):
                 call()
+            with pytest.raises(CdaeError, match="captured"):
+                blk().clip_grad_norm_([other], 1.0, error_if_nonfinite=True)
             with torch.no_grad():
                 call()
         g.replay()

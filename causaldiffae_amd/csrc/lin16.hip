@@ -84,6 +84,7 @@ struct LinArgs {
     float* slab; int splits, k_per_split;   // splits > 1: partial sums [split][M][N] instead of the epilogue
     int tiles_m, tiles_n;
     int past;                               // the result is larger than the caches: written past them
+    const float* sums; void* db; int sum_rows;      // weight gradient beside the data gradient: the bias gradient's partial sums [sum_rows][M] and db, or NULL
 };
 
 template <class T> struct Mfma;
@@ -356,18 +357,37 @@ __device__ __forceinline__ void lin_tile(const LinArgs& p, const int block, unsi
         asm volatile("" ::: "memory");
     }
 }
+// the column sums of the slope pass's blocks, in order: 32 columns x THREADS / 32 lanes of blocks
+template <class T, int THREADS>
+__device__ __forceinline__ void fold_bias(const float* __restrict__ part, int blocks, int N, T* __restrict__ db, int job, float* sh) {
+    constexpr int Q = THREADS / 32;
+    const int cl = threadIdx.x & 31, q = threadIdx.x >> 5, c = job * 32 + cl;
+    const float* at = part + (c < N ? c : N - 1);
+    float s = 0.f;
+#pragma unroll 4
+    for (int b = q; b < blocks; b += Q) s += at[(long)b * N];
+    sh[q * 33 + cl] = s;
+    __syncthreads();
+    if (q || c >= N) return;
+#pragma unroll
+    for (int i = 1; i < Q; ++i) s += sh[i * 33 + cl];
+    st1(db[c], s);
+}
 template <class T, bool AMC, bool BMC, int BM, int WM, int WN, int SLOTS>
 __global__ __launch_bounds__(64 * WM * WN, 2) void lin_tile_kernel(const LinArgs p) {
     extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
     lin_tile<T, AMC, BMC, BM, BM, WM, WN, SLOTS>(p, blockIdx.x, lds);
 }
 // Both products of a backward pass in one launch: the weight gradient's blocks, then (from a multiple of 8, for the XCDs) the data gradient's.  Each alone
-// leaves CUs without work at its end, or from the beginning.
+// leaves CUs without work at its end, or from the beginning.  So do both together, and the fold of the bias gradient's sums is done there, by the last blocks
+// (8192 x 384 -> 1536, a whole training pass: 76.6 us with the fold in a launch of its own, 74.2 so; behind a lone product that fills all CUs, 8192 x 2048 ->
+// 512, 86.0 and 87.7).
 template <class T, int BM, int WM, int WN, int SLOTS>
-__global__ __launch_bounds__(64 * WM * WN, 2) void lin_pair_kernel(const LinArgs pw, const LinArgs px, const int blocks_w) {
+__global__ __launch_bounds__(64 * WM * WN, 2) void lin_pair_kernel(const LinArgs pw, const LinArgs px, const int blocks_w, const int bias_from) {
     extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
     const int second = (blocks_w + 7) & ~7, block = blockIdx.x;
-    if (block < blocks_w) lin_tile<T, true, true, BM, BM, WM, WN, SLOTS>(pw, block, lds);
+    if (block >= bias_from) fold_bias<T, 64 * WM * WN>(pw.sums, pw.sum_rows, pw.M, reinterpret_cast<T*>(pw.db), block - bias_from, reinterpret_cast<float*>(lds));
+    else if (block < blocks_w) lin_tile<T, true, true, BM, BM, WM, WN, SLOTS>(pw, block, lds);
     else if (block >= second) lin_tile<T, false, true, BM, BM, WM, WN, SLOTS>(px, block - second, lds);
 }
 
@@ -479,21 +499,10 @@ __global__ __launch_bounds__(256) void lin_slope_kernel(const T* __restrict__ dy
         else part[(long)rb * N + cc] = t;
     }
 }
-// the column sums of the blocks, in order: 32 columns x 32 lanes of blocks
 template <class T>
 __global__ __launch_bounds__(1024) void lin_bias_kernel(const float* __restrict__ part, int blocks, int N, T* __restrict__ db) {
-    __shared__ float sh[32][33];
-    const int cl = threadIdx.x & 31, q = threadIdx.x >> 5, c = blockIdx.x * 32 + cl;
-    const float* at = part + (c < N ? c : N - 1);
-    float s = 0.f;
-#pragma unroll 4
-    for (int b = q; b < blocks; b += 32) s += at[(long)b * N];
-    sh[q][cl] = s;
-    __syncthreads();
-    if (q || c >= N) return;
-#pragma unroll
-    for (int i = 1; i < 32; ++i) s += sh[i][cl];
-    st1(db[c], s);
+    __shared__ float sh[32 * 33];
+    fold_bias<T, 1024>(part, blocks, N, db, blockIdx.x, sh);
 }
 
 long up8(long v) { return (v + 7) / 8 * 8; }
@@ -508,31 +517,34 @@ size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 //     64 x 64, two blocks a CU                     0.38  3.5    2048 x 1024 -> 1024 forward, 512 tiles of 16 stages: 8.4 us (128 x 128 11.4)
 // A split costs a second launch (3.5) and its partial sums twice (6 TB/s): 1536 x 384 over 8192 rows 26.8 us in seven splits, 64.1 in one, 36.5 in
 // fourteen; 2048 x 1024 over 1024 rows 11.2 in one, 16.8 in two.
+// (A call works its plan out anew, twice with the question for the workspace, so this is host time of every call: tables first, then the combinations.)
 struct Kind { int bm, slots, at_once; double stage, ends; };
 const Kind kinds[] = {{256, 2, 256, 1.5, 9.0}, {128, 4, 256, 0.5, 3.0}, {128, 2, 512, 1.03, 2.7}, {64, 4, 256, 0.26, 2.5}, {64, 4, 512, 0.38, 3.5}};
-bool kind_allowed(const Kind& k) {
-    const int only = cdae_tune(TUNE_LIN16_TILE);
-    return !only || (k.bm == kinds[only - 1].bm && k.slots == kinds[only - 1].slots);
-}
+struct Forced {                              // (tests)
+    int tile = cdae_tune(TUNE_LIN16_TILE), splits = cdae_tune(TUNE_LIN16_SPLITS);
+    bool kind(const Kind& k) const { return !tile || (k.bm == kinds[tile - 1].bm && k.slots == kinds[tile - 1].slots); }
+    bool split(int K, int s) const { return splits ? s == splits : s == 1 || K >= 256 * s; }
+};
 long tiles_of(const Kind& k, int M, int N) { return ((M + k.bm - 1L) / k.bm) * ((N + k.bm - 1L) / k.bm); }
-double block_cost(const Kind& k, int K, int s) { return (double)(((K + s - 1) / s + 63) / 64) * k.stage + k.ends; }
+int stages_of(int K, int s) { return ((K + s - 1) / s + 63) / 64; }
 double split_cost(int M, int N, int s) { return s > 1 ? 3.5 + 8.0 * s * M * N / 6e6 : 0.0; }
-bool split_allowed(int K, int s) {
-    const int forced = cdae_tune(TUNE_LIN16_SPLITS);
-    return forced ? s == forced : s == 1 || K / s >= 256;
-}
 size_t slab_of(int M, int N, int s) { return s > 1 ? up256((size_t)s * M * N * 4) : 0; }
 
 struct Plan { int bm, slots, splits; double cost; };
 Plan plan(int M, int N, int K) {
     static const int splits[] = {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 28, 32, 48, 64};
+    const Forced forced;
     Plan best{256, 2, 1, 1e30};
-    for (const Kind& k : kinds) {
-        const long tiles = tiles_of(k, M, N);
-        if (!kind_allowed(k) || tiles > (1L << 22)) continue;
-        for (int s : splits) {
-            if (!split_allowed(K, s) || (s > 1 && tiles * s > k.at_once && !cdae_tune(TUNE_LIN16_SPLITS))) continue;
-            const double rounds = (double)((tiles * s + k.at_once - 1) / k.at_once), cost = rounds * block_cost(k, K, s) + split_cost(M, N, s);
+    long tiles[5];
+    for (int i = 0; i < 5; ++i) tiles[i] = forced.kind(kinds[i]) ? tiles_of(kinds[i], M, N) : 1L << 40;
+    for (int s : splits) {
+        if (!forced.split(K, s)) continue;
+        const int stages = stages_of(K, s);
+        const double extra = split_cost(M, N, s);
+        for (int i = 0; i < 5; ++i) {
+            const Kind& k = kinds[i];
+            if (tiles[i] > (1L << 22) || (s > 1 && tiles[i] * s > k.at_once && !forced.splits)) continue;
+            const double cost = (double)((tiles[i] * s + k.at_once - 1) / k.at_once) * (stages * k.stage + k.ends) + extra;
             if (cost < best.cost) best = {k.bm, k.slots, s, cost};
         }
     }
@@ -541,30 +553,39 @@ Plan plan(int M, int N, int K) {
 // A backward's two products: dx [M][K] over N, dw [N][K] over M, each by its own plan, or together on one kind of tile where that is cheaper by the same
 // model (a launch that keeps all slots busy takes its blocks' time over the slots, and half a block for its end).
 // 8192 x 384 -> 1536: 36 us together, 49 one after the other (traced).
-struct Pair { bool together; int bm, slots, sx, sw; };
+struct Pair { Plan x, w; bool together; int bm, slots, sx, sw; };
 Pair pair_plan(int M, int N, int K) {
-    static const int splits[] = {1, 2, 3, 4, 6, 8, 12, 16};
-    Pair best{false, 0, 0, 1, 1};
-    double least = plan(M, K, N).cost + plan(N, K, M).cost + 2.5;
+    constexpr int S = 8;
+    static const int splits[S] = {1, 2, 3, 4, 6, 8, 12, 16};
+    const Forced forced;
+    Pair best{plan(M, K, N), plan(N, K, M), false, 0, 0, 1, 1};
+    double least = best.x.cost + best.w.cost + 2.5, ex[S], ew[S];
+    int px[S], pw[S];                                                     // stages; 0: not allowed
+    for (int i = 0; i < S; ++i) {
+        px[i] = forced.split(N, splits[i]) ? stages_of(N, splits[i]) : 0;
+        pw[i] = forced.split(M, splits[i]) ? stages_of(M, splits[i]) : 0;
+        ex[i] = split_cost(M, K, splits[i]);
+        ew[i] = split_cost(N, K, splits[i]);
+    }
     for (const Kind& k : kinds) {
         const long tx = tiles_of(k, M, K), tw = tiles_of(k, N, K);
-        if (!kind_allowed(k) || tx + tw > (1L << 21)) continue;
-        for (int sx : splits) {
-            if (!split_allowed(N, sx)) continue;
-            const double cx = block_cost(k, N, sx), ex = split_cost(M, K, sx);
-            for (int sw : splits) {
-                if (!split_allowed(M, sw)) continue;
-                const double cw = block_cost(k, M, sw), longest = cx > cw ? cx : cw, busy = ((double)tx * sx * cx + (double)tw * sw * cw) / k.at_once;
-                const double cost = (tx * sx + tw * sw <= k.at_once ? longest : busy + 0.5 * longest) + ex + split_cost(N, K, sw);
-                if (cost < least) { least = cost; best = {true, k.bm, k.slots, sx, sw}; }
+        if (!forced.kind(k) || tx + tw > (1L << 21)) continue;
+        for (int i = 0; i < S; ++i) {
+            if (!px[i]) continue;
+            const double cx = px[i] * k.stage + k.ends, nx = (double)tx * splits[i];
+            if (cx + ex[i] >= least) continue;
+            for (int j = 0; j < S; ++j) {
+                if (!pw[j]) continue;
+                const double cw = pw[j] * k.stage + k.ends, nw = (double)tw * splits[j], longest = cx > cw ? cx : cw;
+                const double cost = (nx + nw <= k.at_once ? longest : (nx * cx + nw * cw) / k.at_once + 0.5 * longest) + ex[i] + ew[j];
+                if (cost < least) { least = cost; best.together = true; best.bm = k.bm; best.slots = k.slots; best.sx = splits[i]; best.sw = splits[j]; }
             }
         }
     }
     return best;
 }
-size_t bwd_ws(int M, int N, int K) {
-    const Pair b = pair_plan(M, N, K);
-    const size_t x = slab_of(M, K, plan(M, K, N).splits), w = slab_of(N, K, plan(N, K, M).splits), one = x > w ? x : w;
+size_t bwd_ws(const Pair& b, int M, int N, int K) {
+    const size_t x = slab_of(M, K, b.x.splits), w = slab_of(N, K, b.w.splits), one = x > w ? x : w;
     const size_t both = b.together ? slab_of(M, K, b.sx) + slab_of(N, K, b.sw) : 0;
     return one > both ? one : both;                                       // (a call may want one product only)
 }
@@ -642,12 +663,12 @@ int launch_pair(const LinArgs& pw, const LinArgs& px, long blocks_w, long blocks
     static std::atomic<unsigned long long> done{0};
     auto* kernel = &lin_pair_kernel<T, BM, WM, WN, SLOTS>;
     if (allow_lds(reinterpret_cast<const void*>(kernel), smem, done)) return -1;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((blocks_w + 7) / 8 * 8 + blocks_x)), dim3(64 * WM * WN), smem, st, pw, px, (int)blocks_w);
+    const long bias_from = (blocks_w + 7) / 8 * 8 + blocks_x;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(bias_from + (pw.db ? (pw.M + 31) / 32 : 0))), dim3(64 * WM * WN), smem, st, pw, px, (int)blocks_w, (int)bias_from);
     return hipGetLastError() == hipSuccess ? 0 : cdae_fail("lin16: launch failed");
 }
 template <class T, bool AMC, bool BMC>
-int product(LinArgs p, char* ws, hipStream_t st) {
-    const Plan pl = plan(p.M, p.N, p.K);
+int product(LinArgs p, const Plan& pl, char* ws, hipStream_t st) {
     const long g = lay_out<AMC, BMC>(p, pl.bm, pl.splits, ws);
     if (g < 0) return -1;
     if (pl.bm == 256 ? launch_tiles<T, AMC, BMC, 256, 2, 4, 2>(p, g, st)
@@ -659,9 +680,8 @@ int product(LinArgs p, char* ws, hipStream_t st) {
 }
 // px: dx [M][K] over N;  pw: dw [N][K] over M
 template <class T>
-int products(LinArgs px, LinArgs pw, char* ws, hipStream_t st) {
-    const Pair pl = pair_plan(px.M, px.K, px.N);
-    if (!pl.together) return product<T, false, true>(px, ws, st) || product<T, true, true>(pw, ws, st) ? -1 : 0;
+int products(LinArgs px, LinArgs pw, const Pair& pl, char* ws, hipStream_t st) {
+    if (!pl.together) return product<T, false, true>(px, pl.x, ws, st) || product<T, true, true>(pw, pl.w, ws, st) ? -1 : 0;
     const long gx = lay_out<false, true>(px, pl.bm, pl.sx, ws), gw = lay_out<true, true>(pw, pl.bm, pl.sw, ws + slab_of(px.M, px.N, pl.sx));
     if (gx < 0 || gw < 0) return -1;
     if (pl.bm == 256 ? launch_pair<T, 256, 2, 4, 2>(pw, px, gw, gx, st)
@@ -687,12 +707,20 @@ int slope_rows(int M, int N) {           // rows of a block of the slope pass: a
     const int rows = (int)(((long)M + rb - 1) / rb);
     return rows < 32 ? 32 : (rows + 7) / 8 * 8;
 }
+int slope_blocks(int M, int N) { return (M + slope_rows(M, N) - 1) / slope_rows(M, N); }
 template <class T>
-void slope_launch(const void* dy, long lddy, const void* z, long ldz, u16* dz, float* part, void* dbias, int M, int N, int act, hipStream_t st) {
-    const int ncb = (N + 255) / 256, rows = slope_rows(M, N), rb = (M + rows - 1) / rows;
+void slope_launch(const void* dy, long lddy, const void* z, long ldz, u16* dz, float* part, void* dbias, bool fold, int M, int N, int act, hipStream_t st) {
+    const int ncb = (N + 255) / 256, rows = slope_rows(M, N), rb = slope_blocks(M, N);
     auto* kernel = N < 8 ? &lin_slope_kernel<T, true> : &lin_slope_kernel<T, false>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)(ncb * rb)), dim3(256), 0, st, (const T*)dy, lddy, (const F16*)z, ldz, (T*)dz, up8(N), part, rb == 1 ? (T*)dbias : nullptr, M, N, rows, ncb, act);
-    if (dbias && rb > 1) hipLaunchKernelGGL((lin_bias_kernel<T>), dim3((N + 31) / 32), dim3(1024), 0, st, part, rb, N, (T*)dbias);
+    if (dbias && rb > 1 && fold) hipLaunchKernelGGL((lin_bias_kernel<T>), dim3((N + 31) / 32), dim3(1024), 0, st, part, rb, N, (T*)dbias);
+}
+
+// scratch: copies of operands that cannot be read as they lie, partial sums of the splits; backward: dz and the bias gradient's partial sums too
+size_t copies_of(int lies, int M, int N, int K) { return lies ? 0 : up256((size_t)M * up8(K) * 2) + up256((size_t)N * up8(K) * 2); }
+size_t fwd_bytes(const Plan& pl, int lies, int M, int N, int K) { return copies_of(lies, M, N, K) + slab_of(M, N, pl.splits) + 256; }
+size_t bwd_bytes(const Pair& pl, int lies, int M, int N, int K) {
+    return up256((size_t)M * up8(N) * 2) + up256(sizeof(float) * (size_t)N * slope_blocks(M, N)) + copies_of(lies, M, N, K) + bwd_ws(pl, M, N, K) + 256;
 }
 
 }  // namespace
@@ -701,15 +729,9 @@ extern "C" {
 
 size_t cdae_lin16_workspace_bytes(int op, int M, int N, int K) {
     if (M <= 0 || N <= 0 || K <= 0) return 0;
-    const bool copies = !(op & CDAE_LIN16_ALIGNED);
-    const size_t x = copies ? up256((size_t)M * up8(K) * 2) : 0, w = copies ? up256((size_t)N * up8(K) * 2) : 0;
     switch (op & ~CDAE_LIN16_ALIGNED) {
-        case CDAE_LIN16_FWD: return x + w + slab_of(M, N, plan(M, N, K).splits) + 256;
-        case CDAE_LIN16_BWD: {
-            const int rows = slope_rows(M, N);
-            const size_t sums = up256(sizeof(float) * (size_t)N * ((M + rows - 1) / rows)), most = w + x + bwd_ws(M, N, K);
-            return up256((size_t)M * up8(N) * 2) + (sums > most ? sums : most) + 256;
-        }
+        case CDAE_LIN16_FWD: return fwd_bytes(plan(M, N, K), op & CDAE_LIN16_ALIGNED, M, N, K);
+        case CDAE_LIN16_BWD: return bwd_bytes(pair_plan(M, N, K), op & CDAE_LIN16_ALIGNED, M, N, K);
         default: return 0;
     }
 }
@@ -721,7 +743,8 @@ int cdae_lin16_fwd(const void* x, long ldx, const void* w, long ldw, const void*
     if (M == 0) return 0;
     if (!x || !w || !y || ldx < K || ldw < K || ldy < N || (res && ldres < N) || (z && ldz < N)) return cdae_fail("lin16_fwd: x, w, y and row pitches of at least a row required");
     const int lies = as_it_lies(x, ldx, K) && as_it_lies(w, ldw, K) ? CDAE_LIN16_ALIGNED : 0;
-    if (!ws || !al16(ws) || ws_bytes < cdae_lin16_workspace_bytes(CDAE_LIN16_FWD | lies, M, N, K)) return cdae_fail("lin16_fwd: workspace of cdae_lin16_workspace_bytes() required");
+    const Plan pl = plan(M, N, K);
+    if (!ws || !al16(ws) || ws_bytes < fwd_bytes(pl, lies, M, N, K)) return cdae_fail("lin16_fwd: workspace of cdae_lin16_workspace_bytes() required");
     hipStream_t st = (hipStream_t)stream;
     const Timed timed(PROF_IGEMM, 2.0 * M * N * K, 2.0 * ((double)M * K + (double)N * K + (double)M * N * (1 + (res != nullptr) + (z != nullptr))), st);
     LinArgs p{};
@@ -730,7 +753,7 @@ int cdae_lin16_fwd(const void* x, long ldx, const void* w, long ldw, const void*
     if (prepare({{&p.A, &p.lda, M, K}, {&p.B, &p.ldb, N, K}}, at, st)) return -1;
     p.M = M; p.N = N; p.K = K;
     p.bias = (const u16*)bias; p.res = (const u16*)res; p.ldres = ldres; p.y = (u16*)y; p.ldy = ldy; p.z = (_Float16*)z; p.ldz = ldz; p.act = act;
-    return dt == DT_BF16 ? product<Bf16, false, false>(p, at, st) : product<F16, false, false>(p, at, st);
+    return dt == DT_BF16 ? product<Bf16, false, false>(p, pl, at, st) : product<F16, false, false>(p, pl, at, st);
 }
 
 int cdae_lin16_bwd(const void* dy, long lddy, const void* x, long ldx, const void* w, long ldw, const void* z, long ldz, void* dx, long lddx, void* dw, long lddw,
@@ -741,33 +764,37 @@ int cdae_lin16_bwd(const void* dy, long lddy, const void* x, long ldx, const voi
     if (!dy || lddy < N || (act != L_NONE && (!z || ldz < N))) return cdae_fail("lin16_bwd: dy, and z with an activation, required");
     if ((dx && (!w || ldw < K || lddx < K)) || (dw && (!x || ldx < K || lddw < K))) return cdae_fail("lin16_bwd: w for dx, x for dw, row pitches of at least a row");
     const int lies = (!dx || as_it_lies(w, ldw, K)) && (!dw || as_it_lies(x, ldx, K)) ? CDAE_LIN16_ALIGNED : 0;
-    if (!ws || !al16(ws) || ws_bytes < cdae_lin16_workspace_bytes(CDAE_LIN16_BWD | lies, M, N, K)) return cdae_fail("lin16_bwd: workspace of cdae_lin16_workspace_bytes() required");
+    const Pair pl = pair_plan(M, N, K);
+    if (!ws || !al16(ws) || ws_bytes < bwd_bytes(pl, lies, M, N, K)) return cdae_fail("lin16_bwd: workspace of cdae_lin16_workspace_bytes() required");
     hipStream_t st = (hipStream_t)stream;
     const Timed timed(PROF_IGEMM, 2.0 * M * N * K * ((dx != nullptr) + (dw != nullptr)),
                       2.0 * ((double)M * N * (act ? 2 : 1) + (double)M * K * ((dx != nullptr) + (dw != nullptr)) + (double)N * K * ((dx != nullptr) + (dw != nullptr))), st);
     char* at = (char*)ws;
     const bool copy = act != L_NONE || !as_it_lies(dy, lddy, N);
+    const bool together = dx && dw && pl.together;
     u16* dz = nullptr;
+    float* part = nullptr;
     if (copy && (dx || dw)) { dz = (u16*)at; at += up256((size_t)M * up8(N) * 2); }
     if (dz || dbias) {
-        float* part = dbias ? (float*)at : nullptr;
-        if (dt == DT_BF16) slope_launch<Bf16>(dy, lddy, z, ldz, dz, part, dbias, M, N, act, st);
-        else slope_launch<F16>(dy, lddy, z, ldz, dz, part, dbias, M, N, act, st);
+        part = dbias ? (float*)at : nullptr;
+        if (dbias) at += up256(sizeof(float) * (size_t)N * slope_blocks(M, N));
+        if (dt == DT_BF16) slope_launch<Bf16>(dy, lddy, z, ldz, dz, part, dbias, !together, M, N, act, st);
+        else slope_launch<F16>(dy, lddy, z, ldz, dz, part, dbias, !together, M, N, act, st);
         if (hipGetLastError() != hipSuccess) return cdae_fail("lin16_bwd: launch failed");
     }
     const u16* d = dz ? dz : (const u16*)dy;
     const long ldd = dz ? up8(N) : lddy;
-    // (a stream's launches run in order: the sums of the bias and the products use the same scratch one after the other, but the copies stay)
     LinArgs px{}, pw{};
+    if (dbias && together && slope_blocks(M, N) > 1) { pw.sums = part; pw.sum_rows = slope_blocks(M, N); pw.db = dbias; }
     px.A = pw.A = d; px.lda = pw.lda = ldd;
     px.B = (const u16*)w; px.ldb = ldw; pw.B = (const u16*)x; pw.ldb = ldx;
     px.M = M; px.N = K; px.K = N; px.y = (u16*)dx; px.ldy = lddx;
     pw.M = N; pw.N = K; pw.K = M; pw.y = (u16*)dw; pw.ldy = lddw;
     const Operand ow{&px.B, &px.ldb, N, K}, ox{&pw.B, &pw.ldb, M, K};
     if (dx && dw ? prepare({ow, ox}, at, st) : dx ? prepare({ow}, at, st) : dw ? prepare({ox}, at, st) : 0) return -1;
-    if (dx && dw) return dt == DT_BF16 ? products<Bf16>(px, pw, at, st) : products<F16>(px, pw, at, st);
-    if (dx && (dt == DT_BF16 ? product<Bf16, false, true>(px, at, st) : product<F16, false, true>(px, at, st))) return -1;
-    if (dw && (dt == DT_BF16 ? product<Bf16, true, true>(pw, at, st) : product<F16, true, true>(pw, at, st))) return -1;
+    if (dx && dw) return dt == DT_BF16 ? products<Bf16>(px, pw, pl, at, st) : products<F16>(px, pw, pl, at, st);
+    if (dx && (dt == DT_BF16 ? product<Bf16, false, true>(px, pl.x, at, st) : product<F16, false, true>(px, pl.x, at, st))) return -1;
+    if (dw && (dt == DT_BF16 ? product<Bf16, true, true>(pw, pl.w, at, st) : product<F16, true, true>(pw, pl.w, at, st))) return -1;
     return 0;
 }
 

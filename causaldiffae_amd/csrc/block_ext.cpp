@@ -287,8 +287,14 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         bool want[T_COUNT];
         for (size_t i = 0, edge = 0; i < T_COUNT; ++i) want[i] = t[i].defined() && ctx->needs_input_grad(edge++);
         for (int i : {T_X, T_F}) if (want[i]) g[i] = fresh(t[i].sizes(), t[i]);
-        together(t, want, T_GATE, T_SHIFT, g);
-        together(t, want, T_W1, T_B2, g);
+        int vec = -1, weight = -1;
+        for (int i = T_GATE; i < T_COUNT; ++i) if (want[i]) (i < T_W1 ? vec : weight) = i;
+        if (vec >= 0 && weight >= 0 && t[vec].scalar_type() == t[weight].scalar_type()) {
+            together(t, want, T_GATE, T_B2, g);
+        } else {
+            together(t, want, T_GATE, T_SHIFT, g);
+            together(t, want, T_W1, T_B2, g);
+        }
         if (none) for (int i = T_GATE; i < T_COUNT; ++i) if (g[i].defined()) g[i].zero_();
         if (none) return once(std::move(g));
         const Rows x = rows_of(t[T_X], c.C), f = rows_of(t[T_F], c.C), dr = rows_of(dr_, c.C), du = rows_of(du_, c.C);

@@ -140,7 +140,9 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x_, const Tensor& w_, const std::optional<Tensor>& b, const std::optional<Tensor>& res, int64_t act) {
         const Rows x = rows_of(x_, w_.size(1)), w = rows_of(w_, w_.size(1));
         Tensor z;
-        const bool products = ctx->needs_input_grad(0) || ctx->needs_input_grad(1) || (b && ctx->needs_input_grad(2));
+        // By the tensors alone: ctx->needs_input_grad asks the backward that is running, if one is, so that a forward recomputed inside a backward over
+        // some of the inputs would keep nothing for a later one over others.
+        const bool products = x_.requires_grad() || w_.requires_grad() || (b && b->requires_grad());
         Tensor y = linear_forward(x, w, of(b), of(res), (int)act, products && act ? &z : nullptr, x_);
         if (products) ctx->save_for_backward({x.t, w.t, z});
         ctx->saved_data["act"] = act;
@@ -156,6 +158,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
         if (res && ctx->needs_input_grad(bias ? 3 : 2)) g[3] = dy_;
         if (!ctx->needs_input_grad(0) && !ctx->needs_input_grad(1) && !want_b) return once(std::move(g));
         const variable_list saved = ctx->get_saved_variables();
+        REFUSE(saved.size() == 3, "linear_act: the forward kept nothing for this backward");
         const Tensor &xt = saved[0], &wt = saved[1], &z = saved[2];
         const int64_t K = wt.size(1), N = wt.size(0), M = xt.numel() / K;
         c10::DeviceGuard on(xt.device());

@@ -849,3 +849,58 @@ def test_clip_long():
     assert float(blk().grad_norm([g])) == 5.0
     assert float(blk().clip_grad_norm_([g], 2.5)) == 5.0
     assert float(g[-1]) == 1.5 and float(g[5]) == 2.0
+
+
+# ----------------------------------------------------------------------------- recomputed forwards
+class Recomputed(torch.autograd.Function):
+    """a checkpoint that recomputes its function and differentiates it inside its own backward"""
+
+    @staticmethod
+    def forward(ctx, fn, *inputs):
+        ctx.fn = fn
+        ctx.save_for_backward(*inputs)
+        with torch.no_grad():
+            return fn(*inputs)
+
+    @staticmethod
+    def backward(ctx, dy):
+        with torch.enable_grad():
+            leaves = [t.detach().requires_grad_() for t in ctx.saved_tensors]
+            y = ctx.fn(*leaves)
+        return (None, *torch.autograd.grad(y, leaves, dy))
+
+
+def two_layers(act):
+    args = [rnd(1, 30, 24, dtype=BF16), rnd(2, 40, 24, dtype=BF16, scale=0.2), rnd(3, 40, dtype=BF16), rnd(4, 16, 40, dtype=BF16, scale=0.2)]
+    fn = lambda x, w1, b1, w2: blk().linear_act(blk().linear_act(x, w1, b1, act=act), w2, act=act)
+    return fn, [t.requires_grad_() for t in args], rnd(5, 30, 16, dtype=BF16)
+
+
+@pytest.mark.parametrize("act", ["gelu", "none"])
+def test_linear_act_in_a_checkpoint(act):
+    """the package's checkpoint recomputes the forward inside a backward that was asked for some inputs only"""
+    from causaldiffae_amd.nn import checkpoint
+    fn, leaves, dy = two_layers(act)
+    want = torch.autograd.grad(fn(*leaves), leaves, dy)
+    for pick in ([0], [1], [3], [0, 1, 2, 3]):
+        got = torch.autograd.grad(checkpoint(fn, leaves, (), True), [leaves[i] for i in pick], dy)
+        assert all(torch.equal(g, want[i]) for g, i in zip(got, pick))
+
+
+@pytest.mark.parametrize("act", ["gelu", "none"])
+def test_linear_act_recomputed_with_a_backward_of_its_own(act):
+    fn, leaves, dy = two_layers(act)
+    want = torch.autograd.grad(fn(*leaves), leaves, dy)
+    for pick in ([0], [3], [0, 1, 2, 3]):
+        got = torch.autograd.grad(Recomputed.apply(fn, *leaves), [leaves[i] for i in pick], dy)
+        assert all(torch.equal(g, want[i]) for g, i in zip(got, pick))
+
+
+def test_residual_norm_in_a_checkpoint():
+    from causaldiffae_amd.nn import checkpoint
+    fn = lambda x, w: blk().residual_norm(x, x, pre=w)[1]
+    leaves, dy = [rnd(1, 9, 40).requires_grad_(), rnd(2, 40).requires_grad_()], rnd(3, 9, 40)
+    want = torch.autograd.grad(fn(*leaves), leaves, dy)
+    for i in range(2):
+        for run in (lambda: checkpoint(fn, leaves, (), True), lambda: Recomputed.apply(fn, *leaves)):
+            assert torch.equal(torch.autograd.grad(run(), leaves[i], dy)[0], want[i])

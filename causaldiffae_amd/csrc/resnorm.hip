@@ -230,8 +230,8 @@ __global__ __launch_bounds__(block_of(TPR)) void rn_fwd_kernel(const RnArgs a) {
     const Cols<SMALL> k(threadIdx.x & (TPR - 1), p.C);
     const float inv_c = 1.f / (float)p.C;
     const long chunks = (long)p.B * a.nch;
+    RowSum<TPR> rows(sh);                        // (one for all chunks: the buffers have to go on taking turns where a chunk holds an odd number of sums)
     for (long c = (long)blockIdx.x * GROUPS + threadIdx.x / TPR; c < chunks; c += (long)gridDim.x * GROUPS) {      // (one group a block where there are barriers)
-        RowSum<TPR> rows(sh);
         const long b = c / a.nch;
         const int t0 = (int)(c - b * a.nch) * a.rows_per_chunk, t1 = t0 + a.rows_per_chunk < p.T ? t0 + a.rows_per_chunk : p.T;
         float gw[RN_V], gb[RN_V], sw[RN_V], sb[RN_V];

@@ -904,3 +904,17 @@ def test_residual_norm_in_a_checkpoint():
     for i in range(2):
         for run in (lambda: checkpoint(fn, leaves, (), True), lambda: Recomputed.apply(fn, *leaves)):
             assert torch.equal(torch.autograd.grad(run(), leaves[i], dy)[0], want[i])
+
+
+# ----------------------------------------------------------------------------- more samples than a launch has blocks
+@pytest.mark.parametrize("kind,T", [("layer", 1), ("rms", 1), ("layer", 3)])
+def test_residual_norm_more_samples_than_blocks(kind, T):
+    """blocks that walk several chunks of an odd number of sums (one norm, one or three rows a sample), against the same samples in calls of one chunk a block"""
+    B, C, part = (1 << 20) + 5, 520, 1 << 18
+    g = torch.Generator(device=DEV).manual_seed(7)
+    x = torch.randn(B, T, C, generator=g, device=DEV, dtype=BF16)
+    scale = torch.randn(B, C, generator=g, device=DEV, dtype=BF16)
+    w = 1 + rnd(1, C, dtype=BF16, scale=0.1)
+    got = blk().residual_norm(x, pre=w, scale=scale, kind=kind)[1]
+    for b in range(0, B, part):
+        assert torch.equal(got[b:b + part], blk().residual_norm(x[b:b + part], pre=w, scale=scale[b:b + part], kind=kind)[1]), b

@@ -74,6 +74,7 @@ __device__ __forceinline__ float slope_of(float z) {
     }
 // The pre-activation is kept for the backward in f16 whatever the rows' type: its 11 bits cost the slope a quarter of what the rounding of dz to
 // bf16 costs.  Beyond f16's range it becomes infinite, and the slope there is taken at the range's end, where every slope has long reached its limit.
+// Below that range it becomes zero, where every slope but ReLU's is continuous: finish_row keeps ReLU's positive values positive.
 __device__ __forceinline__ float kept_z(F16 v) { const float z = ld1(v); return fabsf(z) > 65504.f ? copysignf(65504.f, z) : z; }
 
 struct LinArgs {
@@ -110,6 +111,9 @@ __device__ __forceinline__ void finish_row(const LinArgs& p, long m, int n0, int
         Pack<F16, V> k;
 #pragma unroll
         for (int i = 0; i < V; ++i) k.v[i].h = (_Float16)v[i];
+        if (p.act == L_RELU)                                               // (its slope jumps at zero: what is above stays above, as f16's smallest number)
+#pragma unroll
+            for (int i = 0; i < V; ++i) if (v[i] > 0.f) k.v[i].h = (_Float16)fmaxf(v[i], 0x1p-24f);
         if (n >= V) store_past(reinterpret_cast<Pack<F16, V>*>(zp), k);    // (the backward reads it, long after)
         else
 #pragma unroll

@@ -578,7 +578,8 @@ int cdae_wprep_all_m16(const float* flat, const void* desc, int nw, int total_ti
    one call at a time. */
 /* y[M][N] = act(x[M][K] @ w[N][K]^T + bias) + res on 16-bit rows, fp32 accumulation, one rounding (lin16.hip).  Operands of one 16-bit type at any
    pitch >= a row and any alignment; bias [N] and res [M][N] may be NULL.  act: 0 none, 1 SiLU, 3 ReLU, 5 GELU, 6 GELU in its tanh form.  z (may be
-   NULL; for the backward) receives the pre-activation as fp16 whatever dt is (beyond fp16's range: infinity, whose slope is taken at the range's end).
+   NULL; for the backward) receives the pre-activation as fp16 whatever dt is (beyond fp16's range: infinity, whose slope is taken at the range's end; with
+   ReLU a positive one stays positive, fp16's smallest number at least).
    cdae_lin16_bwd: dx = dz @ w, dw = dz^T @ x, dbias = column sums of dz with dz = dy * act'(z) (rounded to the rows' type as an operand of the
    products; the sums take it unrounded); each result may be NULL.  The gradient of res is dy itself. */
 /* workspace: with CDAE_LIN16_ALIGNED added to the operation x and w are 16-byte aligned, K is a multiple of 8 and so are their pitches, which are

@@ -918,3 +918,19 @@ def test_residual_norm_more_samples_than_blocks(kind, T):
     got = blk().residual_norm(x, pre=w, scale=scale, kind=kind)[1]
     for b in range(0, B, part):
         assert torch.equal(got[b:b + part], blk().residual_norm(x[b:b + part], pre=w, scale=scale[b:b + part], kind=kind)[1]), b
+
+
+# ----------------------------------------------------------------------------- activations far below one
+@pytest.mark.parametrize("M,K,N", [(5, 16, 24), (40, 24, 67), (64, 4096, 72), (3, 1, 1)])
+@pytest.mark.parametrize("dtype,xs,ws", [(BF16, 1e-9, 1.0), (BF16, 1e-15, 1e-15), (F16, 1e-4, 1e-5)])
+def test_linear_act_relu_small(M, K, N, dtype, xs, ws):
+    """rows of one sign each with a positive weight, so that every sum has its sign: the slope is 1 on the positive rows however small z is"""
+    sign = 1.0 - 2.0 * (torch.arange(M, device=DEV) % 2)[:, None]
+    x = (sign * xs * (0.5 + rnd(1, M, K).abs()) / K).to(dtype) if dtype == BF16 else (sign * xs * (0.5 + rnd(1, M, K).abs())).to(dtype)
+    w, dy = (ws * (0.5 + rnd(2, N, K).abs())).to(dtype), rnd(3, M, N, dtype=dtype)
+    b = torch.zeros(N, dtype=dtype, device=DEV)
+    x, w, b = (t.requires_grad_() for t in (x, w, b))
+    dx, dw, db = torch.autograd.grad(blk().linear_act(x, w, b, act="relu"), (x, w, b), dy)
+    dz = dy.double() * (sign > 0)
+    for name, g, a, c in (("dx", dx, dz, w.detach().double()), ("dw", dw, dz.t(), x.detach().double()), ("db", db[None], torch.ones(1, M, dtype=torch.float64, device=DEV), dz)):
+        within(name, g, a @ c, (a.shape[1] + 8) * u * (a.abs() @ c.abs()))

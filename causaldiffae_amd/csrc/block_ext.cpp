@@ -63,9 +63,16 @@ Rows rows_of(const Tensor& t, int64_t C) {
 }
 Tensor side_by_side(const Tensor& t) { return !t.defined() || t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
 
+// forward-mode derivatives: a tangent would be lost without a word
+void no_tangent(const char* who, const Tensor& t) { REFUSE(!t.defined() || !t._fw_grad(0).defined(), who, ": there are no forward-mode derivatives"); }
+
 void same_device(const char* who, const Tensor& x, std::initializer_list<Tensor> others) {
     REFUSE(x.is_cuda(), who, ": tensors on an MI355X device required; there is no CPU form");
-    for (const Tensor& t : others) REFUSE(!t.defined() || t.device() == x.device(), who, ": all tensors on one device (", x.device().str(), ")");
+    no_tangent(who, x);
+    for (const Tensor& t : others) {
+        REFUSE(!t.defined() || t.device() == x.device(), who, ": all tensors on one device (", x.device().str(), ")");
+        no_tangent(who, t);
+    }
 }
 bool wanted(std::initializer_list<Tensor> ts) {
     if (!at::GradMode::is_enabled()) return false;
@@ -152,6 +159,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const Tensor& dy_ = grads[0];
+        no_tangent("linear_act", dy_);
         variable_list g(5);
         const bool bias = ctx->saved_data["bias"].toBool(), res = ctx->saved_data["res"].toBool();
         const bool want_b = bias && ctx->needs_input_grad(2);
@@ -285,6 +293,8 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         const bool has_f = t[T_F].defined();
         const Tensor dr_ = has_f ? grads[0] : Tensor(), du_ = c.pre ? grads[has_f ? 1 : 0] : Tensor();
         if (!dr_.defined() && !du_.defined()) return g;
+        no_tangent("residual_norm", dr_);
+        no_tangent("residual_norm", du_);
         const bool none = c.B * c.T == 0;
         c10::DeviceGuard on(t[T_X].device());
         bool want[T_COUNT];
@@ -385,6 +395,7 @@ struct List {
             const Tensor& x = THPVariable_Unpack(h.ptr());
             REFUSE(x.is_cuda() && x.layout() == at::kStrided && type_of(x) >= 0, who, ": dense bf16, fp16 or fp32 tensors on an MI355X device; there is no CPU form");
             REFUSE(t.empty() || x.device() == t[0].device(), who, ": tensors of one device");
+            no_tangent(who, x);
             t.push_back(x);
         }
         dev = t.empty() ? at::Device(at::kCUDA, c10::hip::current_device()) : t[0].device();

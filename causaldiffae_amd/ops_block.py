@@ -11,7 +11,8 @@ Rows are the last dimension: an activation [N, C, H, W] in this package's NHWC s
 Sums, statistics and products accumulate in fp32 (the norm of the gradients in fp64) and every result is rounded once.  Calls run on the current
 stream of their tensors' device, allocate their scratch themselves for the one call, neither synchronise nor copy to the host, keep nothing between
 calls and can be captured into a graph.  (A backward pass can be captured only while no eager graph over the same leaves, made on the default stream,
-is alive: the captured forward raises then.)  Gradients are first derivatives; a second one raises.  Wrong tensors and values raise CdaeError; there is
+is alive: the captured forward raises then.)  Gradients are first derivatives; a second one raises, and so does an input that
+carries a forward-mode tangent.  Wrong tensors and values raise CdaeError; there is
 no CPU form.  The checks and the autograd nodes are native (csrc/block_ext.cpp): the kernels of a call are shorter than the same dispatch from Python.
 """
 import torch

@@ -934,3 +934,25 @@ def test_linear_act_relu_small(M, K, N, dtype, xs, ws):
     dz = dy.double() * (sign > 0)
     for name, g, a, c in (("dx", dx, dz, w.detach().double()), ("dw", dw, dz.t(), x.detach().double()), ("db", db[None], torch.ones(1, M, dtype=torch.float64, device=DEV), dz)):
         within(name, g, a @ c, (a.shape[1] + 8) * u * (a.abs() @ c.abs()))
+
+
+# ----------------------------------------------------------------------------- tensors that are more than their values
+def test_forward_mode_is_refused():
+    """a tangent would be lost without a word"""
+    import torch.autograd.forward_ad as fwad
+    from causaldiffae_amd import CdaeError
+    x, w, v = rnd(1, 6, 16, dtype=BF16), rnd(2, 8, 16, dtype=BF16), rnd(3, 6, 8, dtype=BF16)
+    with fwad.dual_level():
+        dual = lambda t: fwad.make_dual(t, torch.ones_like(t))
+        calls = [lambda: blk().linear_act(dual(x), w), lambda: blk().linear_act(x, dual(w)), lambda: blk().linear_act(x, w, dual(w[:, 0])), lambda: blk().linear_act(x, w, res=dual(v)),
+                 lambda: blk().residual_norm(dual(x), x), lambda: blk().residual_norm(x, dual(x)), lambda: blk().residual_norm(x, x, gate=dual(x[0])),
+                 lambda: blk().residual_norm(x, pre=dual(x[0])), lambda: blk().grad_norm([x, dual(x)]), lambda: blk().clip_grad_norm_([dual(x)], 1.0),
+                 lambda: blk().clip_grad_norm_([x], 1.0, out=[dual(x.clone())])]
+        for call in calls:
+            with pytest.raises(CdaeError, match="forward"):
+                call()
+        assert torch.equal(blk().linear_act(x, w), blk().linear_act(x.clone(), w))
+        a = x.clone().requires_grad_()
+        for y in (blk().linear_act(a, w), *blk().residual_norm(a, x, pre=x[0])):
+            with pytest.raises(RuntimeError, match="forward"):
+                torch.autograd.grad(y, a, dual(torch.ones_like(y)))

@@ -44,9 +44,13 @@ const void* ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nul
 void* mptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor fresh(at::IntArrayRef shape, const Tensor& like) { return at::empty(shape, at::TensorOptions().dtype(like.dtype()).device(like.device())); }
 
+// (a tensor whose values lie negated in memory, until someone asks for them)
+Tensor as_written(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+
 // A tensor [..., C] as rows whose values lie side by side, at a pitch of at least a row: as it lies, or a dense copy
 struct Rows { Tensor t; long pitch; };
-Rows rows_of(const Tensor& t, int64_t C) {
+Rows rows_of(const Tensor& as_given, int64_t C) {
+    const Tensor t = as_written(as_given);
     if (!t.defined()) return {t, 0};
     const int64_t d = t.dim();
     bool ok = C == 1 || t.stride(d - 1) == 1;
@@ -61,7 +65,10 @@ Rows rows_of(const Tensor& t, int64_t C) {
     if (ok || t.numel() == 0) return {t, (long)pitch};
     return {t.contiguous(), (long)C};
 }
-Tensor side_by_side(const Tensor& t) { return !t.defined() || t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+Tensor side_by_side(const Tensor& as_given) {
+    const Tensor t = as_written(as_given);
+    return !t.defined() || t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous();
+}
 
 // forward-mode derivatives: a tangent would be lost without a word
 void no_tangent(const char* who, const Tensor& t) { REFUSE(!t.defined() || !t._fw_grad(0).defined(), who, ": there are no forward-mode derivatives"); }
@@ -130,7 +137,7 @@ Tensor linear_forward(const Rows& x, const Rows& w, const Tensor& b, const Tenso
     Tensor y = fresh(shape, x.t);
     if (z) *z = at::empty({M, N}, x.t.options().dtype(at::kHalf).requires_grad(false));
     if (!M) return y;
-    const Tensor bias = b.defined() ? b.contiguous() : b;
+    const Tensor bias = side_by_side(b);
     const Rows res = rows_of(res_, N);
     const size_t need = linear_scratch(CDAE_LIN16_FWD, x, w, M);
     const Tensor ws = scratch(need, x.t);
@@ -400,7 +407,12 @@ struct List {
         }
         dev = t.empty() ? at::Device(at::kCUDA, c10::hip::current_device()) : t[0].device();
     }
-    void read_dense() { for (Tensor& x : t) if (!dense(x)) x = x.detach().contiguous(); }
+    void read_dense() {
+        for (Tensor& x : t) {
+            x = as_written(x.is_neg() ? x.detach() : x);
+            if (!dense(x)) x = x.detach().contiguous();
+        }
+    }
     void arrays() {
         p.clear(); n.clear(); ty.clear();
         for (const Tensor& x : t) { p.push_back(x.const_data_ptr()); n.push_back((long)x.numel()); ty.push_back(type_of(x)); }
@@ -434,20 +446,21 @@ Tensor clip_grad_norm(const py::object& grads, double max_norm, double scale, co
     List src(who, grads);
     c10::DeviceGuard on(src.dev);
     REFUSE(!error_if_nonfinite || !capturing(src.dev), who, ": error_if_nonfinite waits for the device and cannot be captured");
-    std::vector<std::pair<Tensor, Tensor>> later;              // (tensor with gaps, dense copy): written back at the end
+    std::vector<std::pair<Tensor, Tensor>> later;              // (tensor with gaps or negated, dense copy): written back at the end
     List dst = out.is_none() ? src : List(who, out);
     REFUSE(dst.t.size() == src.t.size(), who, ": an output for every gradient");
     for (size_t i = 0; i < src.t.size(); ++i) {
         Tensor &a = src.t[i], &b = dst.t[i];
         if (out.is_none()) {
-            if (dense(a)) continue;
+            if (dense(a) && !a.is_neg()) continue;
             for (int64_t d = 0; d < a.dim(); ++d) REFUSE(a.size(d) <= 1 || a.stride(d) != 0, who, ": an expanded tensor cannot be written in place");
-            b = a.contiguous();
+            b = as_written(a).contiguous();
             later.emplace_back(a, b);
             a = b;
         } else {
             REFUSE(a.sizes() == b.sizes() && b.device() == src.dev, who, ": outputs of the gradients' shapes, on their device");
-            REFUSE(dense(b), who, ": outputs without gaps");
+            REFUSE(dense(b) && !b.is_neg(), who, ": outputs without gaps, their values as they are");
+            a = as_written(a);
             if (!(a.is_contiguous() && b.is_contiguous()) && !(dense(a) && a.strides() == b.strides())) a = at::empty_strided(b.sizes(), b.strides(), a.options()).copy_(a);
         }
     }

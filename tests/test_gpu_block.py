@@ -956,3 +956,34 @@ def test_forward_mode_is_refused():
         for y in (blk().linear_act(a, w), *blk().residual_norm(a, x, pre=x[0])):
             with pytest.raises(RuntimeError, match="forward"):
                 torch.autograd.grad(y, a, dual(torch.ones_like(y)))
+
+
+def test_tensors_negated_lazily():
+    """a tensor whose values lie negated in memory counts with its values"""
+    neg = torch._neg_view
+    x, f, w = rnd(1, 6, 16, dtype=BF16), rnd(2, 6, 16, dtype=BF16), rnd(3, 8, 16, dtype=BF16)
+    b, res = rnd(4, 8, dtype=BF16), rnd(5, 6, 8, dtype=BF16)
+    for i in range(4):
+        args = [x, w, b, res]
+        args[i] = -args[i]
+        want = blk().linear_act(*args, act="silu")
+        args[i] = neg([x, w, b, res][i])
+        assert args[i].is_neg() and torch.equal(blk().linear_act(*args, act="silu"), want)
+    for k in ("x", "f", "gate", "scale", "pre"):
+        args = {"x": x, "f": f, "gate": x[0], "scale": f[:2], "pre": w[0]}
+        want = blk().residual_norm(**{**args, k: -args[k]})
+        got = blk().residual_norm(**{**args, k: neg(args[k])})
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+    leaf = w.clone().requires_grad_()
+    g, = torch.autograd.grad(blk().linear_act(x, leaf), leaf, neg(res))
+    assert torch.equal(g, torch.autograd.grad(blk().linear_act(x, leaf), leaf, -res)[0])
+    leaf = x.clone().requires_grad_()
+    g, = torch.autograd.grad(blk().residual_norm(leaf, pre=w[0])[1], leaf, neg(f))
+    assert torch.equal(g, torch.autograd.grad(blk().residual_norm(leaf, pre=w[0])[1], leaf, -f)[0])
+    n = exact_norm([x])
+    out = torch.empty(6, 16, device=DEV)
+    blk().clip_grad_norm_([neg(x)], n / 2, out=[out])
+    within("out", out, -x.double() * (n / 2 / (n + 1e-6)), 2 * u * x.double().abs())
+    a = x.clone()
+    blk().clip_grad_norm_([neg(a)], n / 2)
+    within("in place", a, x.double() * (n / 2 / (n + 1e-6)), 2 * u * x.double().abs())

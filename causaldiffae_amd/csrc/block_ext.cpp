@@ -73,10 +73,14 @@ Tensor side_by_side(const Tensor& as_given) {
 // forward-mode derivatives: a tangent would be lost without a word
 void no_tangent(const char* who, const Tensor& t) { REFUSE(!t.defined() || !t._fw_grad(0).defined(), who, ": there are no forward-mode derivatives"); }
 
+bool has_values(const Tensor& t) { return t.layout() == at::kStrided && !t.is_nested() && t.has_storage(); }      // (a sparse or nested tensor's do not lie in rows)
+
 void same_device(const char* who, const Tensor& x, std::initializer_list<Tensor> others) {
     REFUSE(x.is_cuda(), who, ": tensors on an MI355X device required; there is no CPU form");
+    REFUSE(has_values(x), who, ": dense tensors required");
     no_tangent(who, x);
     for (const Tensor& t : others) {
+        REFUSE(!t.defined() || has_values(t), who, ": dense tensors required");
         REFUSE(!t.defined() || t.device() == x.device(), who, ": all tensors on one device (", x.device().str(), ")");
         no_tangent(who, t);
     }
@@ -400,7 +404,7 @@ struct List {
         for (py::handle h : list) {
             REFUSE(THPVariable_Check(h.ptr()), who, ": a list of tensors");
             const Tensor& x = THPVariable_Unpack(h.ptr());
-            REFUSE(x.is_cuda() && x.layout() == at::kStrided && type_of(x) >= 0, who, ": dense bf16, fp16 or fp32 tensors on an MI355X device; there is no CPU form");
+            REFUSE(x.is_cuda() && has_values(x) && type_of(x) >= 0, who, ": dense bf16, fp16 or fp32 tensors on an MI355X device; there is no CPU form");
             REFUSE(t.empty() || x.device() == t[0].device(), who, ": tensors of one device");
             no_tangent(who, x);
             t.push_back(x);

@@ -987,3 +987,14 @@ def test_tensors_negated_lazily():
     a = x.clone()
     blk().clip_grad_norm_([neg(a)], n / 2)
     within("in place", a, x.double() * (n / 2 / (n + 1e-6)), 2 * u * x.double().abs())
+
+
+def test_layouts_are_refused():
+    from causaldiffae_amd import CdaeError
+    x, w = rnd(1, 6, 16), rnd(2, 8, 16, dtype=BF16)
+    sparse = x.relu().to_sparse()
+    for call in (lambda: blk().linear_act(sparse.to(BF16), w), lambda: blk().linear_act(x.to(BF16), w.relu().to_sparse()), lambda: blk().residual_norm(sparse, x), lambda: blk().residual_norm(x, sparse),
+                 lambda: blk().residual_norm(x, pre=x[0].relu().to_sparse()), lambda: blk().grad_norm([sparse]),
+                 lambda: blk().clip_grad_norm_([x], 1.0, out=[torch._neg_view(torch.empty_like(x))])):
+        with pytest.raises(CdaeError):
+            call()

@@ -328,7 +328,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         p.du = ptr(du.t); p.ld_du = du.pitch;
         p.dx = mptr(g[T_X]); p.df = mptr(g[T_F]); p.dgate = mptr(g[T_GATE]); p.dscale = mptr(g[T_SCALE]); p.dshift = mptr(g[T_SHIFT]);
         p.dw1 = mptr(g[T_W1]); p.db1 = mptr(g[T_B1]); p.dw2 = mptr(g[T_W2]); p.db2 = mptr(g[T_B2]);
-        p.ws_bytes = cdae_resnorm_workspace_bytes(p.B, p.T, p.C);
+        p.ws_bytes = vec < 0 && weight < 0 ? 256 : cdae_resnorm_workspace_bytes(p.B, p.T, p.C);
         const Tensor ws = scratch(p.ws_bytes, x.t);
         p.ws = (float*)mptr(ws);
         check(cdae_resnorm_bwd(&p, stream_of(x.t)));

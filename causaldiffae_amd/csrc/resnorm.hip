@@ -40,6 +40,8 @@ constexpr long RN_MAX_GRID = 1 << 20;            // (a launch holds fewer than 2
 constexpr long RN_MAX_BLOCKS = 1 << 22;          // chunks of a backward call: 2^22 x 1024 threads would be the bound itself
 
 constexpr int RN_SUMS = 7;                       // of a sample: g A1, g A2, (1 + s) A3, (1 + s) A4, and the gradients of g, s, t
+constexpr int RN_GROUPS = 1024;                  // groups of samples, of 32 at least, that are folded before their sums are written
+constexpr long RN_SLAB = 1 << 22;                // column sums (of four) that a backward call keeps at a time: 64 MB, or what half a tensor of its 16-bit rows takes
 
 struct RnArgs {
     cdae_resnorm p;
@@ -389,6 +391,7 @@ __global__ __launch_bounds__(block_of(TPR)) void rn_bwd_kernel(const RnArgs a) {
             }
         }
     }
+    if (!p.ws) return;                                            // (no vector has a gradient)
     float* part = p.ws + (long)blockIdx.x * 4 * p.C;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -407,6 +410,28 @@ __global__ __launch_bounds__(block_of(TPR)) void rn_bwd_kernel(const RnArgs a) {
             k.put(part + j * p.C, A[j]);
         }
     }
+}
+
+// Gradients of a sample's own gate, scale and shift in column c from its column sums, written; o: what it gives to the sums that samples share
+template <class T>
+__device__ __forceinline__ void fold_sample(const cdae_resnorm& p, long b, int c, float w1, float b1, float w2, float b2, const float (&A)[4], float (&o)[RN_SUMS]) {
+    auto vec = [&](const void* v, long off, float none) { return !v ? none : p.vec32 ? ((const float*)v)[off] : ld1(((const T*)v)[off]); };
+    const float g = vec(p.gate, (p.shared_gate ? 0 : b * p.ld_gate) + c, 1.f) * p.alpha, s1 = 1.f + vec(p.scale, (p.shared_scale ? 0 : b * p.ld_scale) + c, 0.f);
+    const float dg = p.alpha * (w1 * A[0] + b1 * A[1]), ds = w2 * A[2] + b2 * A[3];
+    if (p.dgate && !p.shared_gate) st2<T>(p.dgate, b * p.C + c, p.vec32, dg);
+    if (p.dscale && !p.shared_scale) st2<T>(p.dscale, b * p.C + c, p.vec32, ds);
+    if (p.dshift && !p.shared_shift) st2<T>(p.dshift, b * p.C + c, p.vec32, A[3]);
+    o[0] = g * A[0]; o[1] = g * A[1]; o[2] = s1 * A[2]; o[3] = s1 * A[3]; o[4] = dg; o[5] = ds; o[6] = A[3];
+}
+template <class T>
+__device__ __forceinline__ float weight_of(const cdae_resnorm& p, const void* v, int c, float none) { return !v ? none : p.w32 ? ((const float*)v)[c] : ld1(((const T*)v)[c]); }
+// where sum j of all samples belongs, or NULL
+__device__ __forceinline__ void* shared_of(const cdae_resnorm& p, int j) {
+    void* const dst[RN_SUMS] = {p.dw1, p.db1, p.dw2, p.db2, p.shared_gate ? p.dgate : nullptr, p.shared_scale ? p.dscale : nullptr, p.shared_shift ? p.dshift : nullptr};
+    void* out = nullptr;
+#pragma unroll
+    for (int i = 0; i < RN_SUMS; ++i) if (i == j) out = dst[i];
+    return out;
 }
 
 // The column sums of each sample from its chunks, and from them the gradients of gate, scale and shift; what the samples
@@ -441,40 +466,58 @@ __global__ __launch_bounds__(1024) void rn_fold_kernel(const RnArgs a, float* __
         if (q || c >= p.C) continue;
 #pragma unroll
         for (int j = 0; j < 4; ++j) A[j] = sh[j][0][cl];
-        auto vec = [&](const void* v, long off, int is32, float none) { return !v ? none : is32 ? ((const float*)v)[off] : ld1(((const T*)v)[off]); };
-        const float g = vec(p.gate, (p.shared_gate ? 0 : b * p.ld_gate) + c, p.vec32, 1.f) * p.alpha, s1 = 1.f + vec(p.scale, (p.shared_scale ? 0 : b * p.ld_scale) + c, p.vec32, 0.f);
-        const float w1 = vec(p.w1, c, p.w32, 1.f), b1 = vec(p.b1, c, p.w32, 0.f), w2 = vec(p.w2, c, p.w32, 1.f), b2 = vec(p.b2, c, p.w32, 0.f);
-        const float dg = p.alpha * (w1 * A[0] + b1 * A[1]), ds = w2 * A[2] + b2 * A[3];
-        if (p.dgate && !p.shared_gate) st2<T>(p.dgate, b * p.C + c, p.vec32, dg);
-        if (p.dscale && !p.shared_scale) st2<T>(p.dscale, b * p.C + c, p.vec32, ds);
-        if (p.dshift && !p.shared_shift) st2<T>(p.dshift, b * p.C + c, p.vec32, A[3]);
-        const float o[RN_SUMS] = {g * A[0], g * A[1], s1 * A[2], s1 * A[3], dg, ds, A[3]};
-        if (p.B == 1) {
-            void* const dst[RN_SUMS] = {p.dw1, p.db1, p.dw2, p.db2, p.shared_gate ? p.dgate : nullptr, p.shared_scale ? p.dscale : nullptr, p.shared_shift ? p.dshift : nullptr};
+        float o[RN_SUMS];
+        fold_sample<T>(p, b, c, weight_of<T>(p, p.w1, c, 1.f), weight_of<T>(p, p.b1, c, 0.f), weight_of<T>(p, p.w2, c, 1.f), weight_of<T>(p, p.b2, c, 0.f), A, o);
 #pragma unroll
-            for (int j = 0; j < RN_SUMS; ++j) if (dst[j]) st2<T>(dst[j], c, j < 4 ? p.w32 : p.vec32, o[j]);
-            continue;
+        for (int j = 0; j < RN_SUMS; ++j) {
+            if (p.B > 1) sums[(b * RN_SUMS + j) * p.C + c] = o[j];
+            else if (void* const out = shared_of(p, j)) st2<T>(out, c, j < 4 ? p.w32 : p.vec32, o[j]);
         }
-#pragma unroll
-        for (int j = 0; j < RN_SUMS; ++j) sums[(b * RN_SUMS + j) * p.C + c] = o[j];
     }
 }
 
-// what all samples share: grid y picks one of the seven sums; 32 columns x 8 lanes of samples
+// The same for samples of one chunk each, `per_group` to a block of 32 columns x 32 lanes of samples: what they share is added up before it is written, to
+// sums[group][7][C] or, for a single group, to the results themselves.
 template <class T>
-__global__ __launch_bounds__(256) void rn_shared_kernel(const RnArgs a, const float* __restrict__ sums) {
+__global__ __launch_bounds__(1024) void rn_fold_samples_kernel(const RnArgs a, float* __restrict__ sums, int per_group, int single) {
     const cdae_resnorm& p = a.p;
+    const int ncb = (p.C + 31) / 32, cl = threadIdx.x & 31, q = threadIdx.x >> 5, group = blockIdx.x / ncb, c = (blockIdx.x - group * ncb) * 32 + cl;
+    __shared__ float sh[RN_SUMS][32][33];
+    float total[RN_SUMS] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (c < p.C) {
+        const float w1 = weight_of<T>(p, p.w1, c, 1.f), b1 = weight_of<T>(p, p.b1, c, 0.f), w2 = weight_of<T>(p, p.w2, c, 1.f), b2 = weight_of<T>(p, p.b2, c, 0.f);
+        const int first = group * per_group, end = first + per_group < p.B ? first + per_group : p.B;
+        for (int b = first + q; b < end; b += 32) {
+            float A[4], o[RN_SUMS];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) A[j] = p.ws[((long)b * 4 + j) * p.C + c];
+            fold_sample<T>(p, b, c, w1, b1, w2, b2, A, o);
+#pragma unroll
+            for (int j = 0; j < RN_SUMS; ++j) total[j] += o[j];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < RN_SUMS; ++j) sh[j][q][cl] = total[j];
+    __syncthreads();
+    if (q >= RN_SUMS || c >= p.C) return;                                 // the threads of q add sum q, in order
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) s += sh[q][i][cl];
+    if (!single) sums[((long)group * RN_SUMS + q) * p.C + c] = s;
+    else if (void* const out = shared_of(p, q)) st2<T>(out, c, q < 4 ? p.w32 : p.vec32, s);
+}
+
+// what all samples share: grid y picks one of the seven sums; 32 columns x 8 lanes of samples or groups of them
+template <class T>
+__global__ __launch_bounds__(256) void rn_shared_kernel(const cdae_resnorm p, const float* __restrict__ sums, int count) {
     const int cl = threadIdx.x & 31, q = threadIdx.x >> 5, c = blockIdx.x * 32 + cl, j = blockIdx.y;
     __shared__ float sh[8][32];
-    void* const dst[RN_SUMS] = {p.dw1, p.db1, p.dw2, p.db2, p.shared_gate ? p.dgate : nullptr, p.shared_scale ? p.dscale : nullptr, p.shared_shift ? p.dshift : nullptr};
-    void* out = nullptr;
-#pragma unroll
-    for (int i = 0; i < RN_SUMS; ++i) if (i == j) out = dst[i];
+    void* const out = shared_of(p, j);
     if (!out) return;                                                     // (block-uniform)
     float s = 0.f;
     const float* at = sums + (long)j * p.C + (c < p.C ? c : p.C - 1);
 #pragma unroll 4
-    for (int b = q; b < p.B; b += 8) s += at[(long)b * RN_SUMS * p.C];
+    for (int b = q; b < count; b += 8) s += at[(long)b * RN_SUMS * p.C];
     sh[q][cl] = s;
     __syncthreads();
     if (q || c >= p.C) return;
@@ -545,21 +588,71 @@ void fwd(const cdae_resnorm* p, hipStream_t st) {
     RN_TPR(RN_CALL)
 #undef RN_CALL
 }
+bool any_vector(const cdae_resnorm* p) { return p->dgate || p->dscale || p->dshift || p->dw1 || p->db1 || p->dw2 || p->db2; }
+bool any_shared(const cdae_resnorm* p) {
+    return p->dw1 || p->db1 || p->dw2 || p->db2 || (p->dgate && p->shared_gate) || (p->dscale && p->shared_scale) || (p->dshift && p->shared_shift);
+}
+// Samples of a group, and samples of a slab: with few rows a sample the four column sums of every sample would be a multiple of the rows themselves (16 bytes
+// a value beside 2), so that such calls go over the samples in slabs, which share one place for them.  More than one slab means one chunk a sample.
+int group_of(int B) { return 32 * (int)((B + 32L * RN_GROUPS - 1) / (32L * RN_GROUPS)); }
+int slab_of(int B, int T, int C) {
+    const long rows = (long)B * T * C / 16, most = (rows > RN_SLAB ? rows : RN_SLAB) / C, per = group_of(B);
+    return most >= B ? B : (int)(most < per ? per : most / per * per);
+}
+size_t sums_at(int B, int T, int C, int nch) { return 4 * (size_t)C * (nch > 1 ? (size_t)B * nch : (size_t)slab_of(B, T, C)); }      // (floats in front of the shared sums)
+size_t scratch_floats(int B, int T, int C, int nch) {
+    return sums_at(B, T, C, nch) + RN_SUMS * (size_t)C * (nch > 1 ? B : (B + group_of(B) - 1) / group_of(B));
+}
+
+// samples from `first` on, `count` of them
+template <class T>
+cdae_resnorm part_of(const cdae_resnorm& whole, long first, int count) {
+    cdae_resnorm p = whole;
+    const long t = first * p.T, vec = p.vec32 ? 4 : sizeof(T);
+    auto in = [](const void*& v, long by) { if (v) v = (const char*)v + by; };
+    auto out = [](void*& v, long by) { if (v) v = (char*)v + by; };
+    p.B = count;
+    in(p.x, t * p.ld_x * sizeof(T)); in(p.f, t * p.ld_f * sizeof(T)); in(p.dr, t * p.ld_dr * sizeof(T)); in(p.du, t * p.ld_du * sizeof(T));
+    out(p.dx, t * p.C * sizeof(T)); out(p.df, t * p.C * sizeof(T));
+    if (!p.shared_gate) { in(p.gate, first * p.ld_gate * vec); out(p.dgate, first * p.C * vec); }
+    if (!p.shared_scale) { in(p.scale, first * p.ld_scale * vec); out(p.dscale, first * p.C * vec); }
+    if (!p.shared_shift) { in(p.shift, first * p.ld_shift * vec); out(p.dshift, first * p.C * vec); }
+    return p;
+}
+template <class T>
+void bwd_rows(const RnArgs& a, hipStream_t st) {
+    const cdae_resnorm* p = &a.p;
+#define RN_CALL(N, S) hipLaunchKernelGGL((rn_bwd_kernel<T, N, S>), dim3((unsigned)((long)p->B * a.nch)), dim3(block_of(N)), 0, st, a)
+    RN_TPR(RN_CALL)
+#undef RN_CALL
+}
 template <class T>
 void bwd(const cdae_resnorm* p, hipStream_t st) {
     RnArgs a;
     a.p = *p;
     chunks_of(p->B, p->T, p->C, sizeof(T) == 4, a.nch, a.rows_per_chunk);
-    float* sums = p->ws + (long)p->B * a.nch * 4 * p->C;
-#define RN_CALL(N, S) hipLaunchKernelGGL((rn_bwd_kernel<T, N, S>), dim3((unsigned)((long)p->B * a.nch)), dim3(block_of(N)), 0, st, a)
-    RN_TPR(RN_CALL)
-#undef RN_CALL
-    if (!(p->dgate || p->dscale || p->dshift || p->dw1 || p->db1 || p->dw2 || p->db2)) return;
-    const long jobs = (p->C + 31L) / 32 * p->B;
-    hipLaunchKernelGGL((rn_fold_kernel<T>), dim3((unsigned)(jobs < RN_MAX_GRID ? jobs : RN_MAX_GRID)), dim3(1024), 0, st, a, sums);
-    if (p->B == 1) return;
-    if (p->dw1 || p->db1 || p->dw2 || p->db2 || (p->dgate && p->shared_gate) || (p->dscale && p->shared_scale) || (p->dshift && p->shared_shift))
-        hipLaunchKernelGGL((rn_shared_kernel<T>), dim3((p->C + 31) / 32, RN_SUMS), dim3(256), 0, st, a, sums);
+    if (!any_vector(p)) {
+        a.p.ws = nullptr;
+        return bwd_rows<T>(a, st);
+    }
+    float* const sums = p->ws + sums_at(p->B, p->T, p->C, a.nch);
+    const int ncb = (p->C + 31) / 32;
+    int count = p->B;                                                     // of the shared sums' parts
+    if (a.nch > 1) {
+        bwd_rows<T>(a, st);
+        const long jobs = (long)ncb * p->B;
+        hipLaunchKernelGGL((rn_fold_kernel<T>), dim3((unsigned)(jobs < RN_MAX_GRID ? jobs : RN_MAX_GRID)), dim3(1024), 0, st, a, sums);
+    } else {
+        const int per = group_of(p->B), slab = slab_of(p->B, p->T, p->C);
+        count = (p->B + per - 1) / per;
+        for (long first = 0; first < p->B; first += slab) {
+            a.p = part_of<T>(*p, first, (int)(p->B - first < slab ? p->B - first : slab));
+            bwd_rows<T>(a, st);
+            hipLaunchKernelGGL((rn_fold_samples_kernel<T>), dim3((unsigned)(ncb * ((a.p.B + per - 1) / per))), dim3(1024), 0, st, a,
+                               sums + first / per * RN_SUMS * p->C, per, count == 1);
+        }
+    }
+    if (count > 1 && any_shared(p)) hipLaunchKernelGGL((rn_shared_kernel<T>), dim3(ncb, RN_SUMS), dim3(256), 0, st, *p, sums, count);
 }
 
 }  // namespace
@@ -571,7 +664,8 @@ size_t cdae_resnorm_workspace_bytes(int B, int T, int C) {
     int nch, nch32, rows;
     chunks_of(B, T, C, false, nch, rows);
     chunks_of(B, T, C, true, nch32, rows);
-    return sizeof(float) * 4 * (size_t)C * B * (nch > nch32 ? nch : nch32) + sizeof(float) * RN_SUMS * (size_t)C * B;
+    const size_t n = scratch_floats(B, T, C, nch), n32 = scratch_floats(B, T, C, nch32);
+    return sizeof(float) * (n > n32 ? n : n32);
 }
 
 int cdae_resnorm_fwd(const cdae_resnorm* p, void* stream) {
@@ -595,7 +689,8 @@ int cdae_resnorm_bwd(const cdae_resnorm* p, void* stream) {
     if ((p->dgate && !p->gate) || (p->dscale && !p->scale) || (p->dshift && !p->shift) || (p->dw1 && !p->w1) || (p->db1 && !p->b1) || (p->dw2 && !p->w2) ||
         (p->db2 && !p->b2))
         return cdae_fail("resnorm_bwd: a gradient of a vector that is not there");
-    if (!p->ws || ((size_t)p->ws & 15) || p->ws_bytes < cdae_resnorm_workspace_bytes(p->B, p->T, p->C)) return cdae_fail("resnorm_bwd: workspace of cdae_resnorm_workspace_bytes() required");
+    if (!p->ws || ((size_t)p->ws & 15) || p->ws_bytes < (any_vector(p) ? cdae_resnorm_workspace_bytes(p->B, p->T, p->C) : 256))
+        return cdae_fail("resnorm_bwd: workspace of cdae_resnorm_workspace_bytes(), or of 256 bytes without gradients of vectors, required");
     hipStream_t st = (hipStream_t)stream;
     const double rows = (double)p->B * p->T * p->C * (p->dt == DT_F32 ? 4 : 2) * (1 + (p->f != nullptr) + (p->dr != nullptr) + (p->du != nullptr) + (p->dx != nullptr) + (p->df != nullptr));
     const Timed timed(PROF_GN, rows, rows, st);

@@ -595,7 +595,8 @@ int cdae_lin16_bwd(const void* dy, long lddy, const void* x, long ldx, const voi
    post and pre: layer norms (layer = 1) or rms norms (0) with weight and bias (w1, b1 / w2, b2: each may be NULL), or absent.  f may be NULL: then
    r = x, and r is not written.  gate, scale, shift: a vector for each sample (a row pitch ld_*), or one for all samples (shared_* = 1), or NULL; fp32
    (vec32 = 1) or the rows' type; w and b likewise (w32).  r, u and the gradients of rows are dense; x, f, dr, du have pitches.
-   Backward: dr and du in (either may be NULL); every output may be NULL.  dgate, dscale and dshift are dense, [B][C], or [C] for a shared vector. */
+   Backward: dr and du in (either may be NULL); every output may be NULL.  dgate, dscale and dshift are dense, [B][C], or [C] for a shared vector.
+   Its workspace: cdae_resnorm_workspace_bytes(), or 256 bytes where no gradient of a vector (gate ... b2) is asked for. */
 typedef struct cdae_resnorm {
     int B, T, C, dt, layer, post, pre, vec32, w32, shared_gate, shared_scale, shared_shift;
     float alpha, eps;

@@ -119,3 +119,9 @@ def test_host_tensors_are_refused():
     for call in (lambda: ops_block.linear_act(x, x), lambda: ops_block.residual_norm(x, x), lambda: ops_block.grad_norm([x]), lambda: ops_block.clip_grad_norm_([x], 1.0)):
         with pytest.raises(CdaeError):
             call()
+
+
+@pytest.mark.parametrize("B,T,C", [(1 << 20, 1, 520), (65536, 1, 1024), (1 << 17, 1, 8192), (9000, 1, 1000), (600, 1, 8192), (1 << 21, 3, 64), (32, 256, 384), (8, 4096, 2048)])
+def test_norm_scratch_stays_beside_the_rows(B, T, C):
+    """with a vector for every row the column sums of all samples would be many times the rows: the backward keeps 64 MB, or less than one tensor of 16-bit rows"""
+    assert 16 * C <= lib.cdae_resnorm_workspace_bytes(B, T, C) <= (64 << 20) + 2 * B * T * C

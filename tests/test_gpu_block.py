@@ -998,3 +998,31 @@ def test_layouts_are_refused():
                  lambda: blk().clip_grad_norm_([x], 1.0, out=[torch._neg_view(torch.empty_like(x))])):
         with pytest.raises(CdaeError):
             call()
+
+
+@pytest.mark.parametrize("B,T,C,dtype,gate,mod", [(9000, 1, 1000, BF16, "sample", "sample"), (20000, 2, 264, F32, "channel", "sample"), (70000, 1, 72, F16, "sample", "channel"),
+                                                  (600, 1, 8192, BF16, "channel", "channel"), (40, 1, 520, F32, "sample", "sample"), (33, 3, 5, BF16, "sample", None)])
+def test_residual_norm_sample_folds(B, T, C, dtype, gate, mod):
+    """few rows a sample: samples folded in groups, and (the first three) in several slabs that share one place for their column sums"""
+    v = vectors(B, C, dtype, gate, mod, True, True)
+    r = lambda s: rnd(s, B, T, C, dtype=dtype)
+    check_norm(r(1), r(2), v, 0.7, True, True, "layer", dr=r(3), du=r(4))
+
+
+def test_residual_norm_without_vector_gradients():
+    """vectors that need no gradient: the gradients of the rows are the same, without the column sums' scratch"""
+    B, T, C = 2000, 1, 4000
+    v = vectors(B, C, BF16, "sample", "sample", True, True)
+    x, f, dr, du = (rnd(s, B, T, C, dtype=BF16) for s in (1, 2, 3, 4))
+    call = lambda: blk().residual_norm(x, f, gate=v["gate"], post=(v["w1"], v["b1"]), pre=(v["w2"], v["b2"]), scale=v["scale"], shift=v["shift"])
+    x.requires_grad_(), f.requires_grad_()
+    outs = call()
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    alone = torch.autograd.grad(outs, (x, f), (dr, du))
+    assert torch.cuda.max_memory_allocated() - before < 3 * x.numel() * 2
+    for t in v.values():
+        t.requires_grad_()
+    both = torch.autograd.grad(call(), (x, f, *v.values()), (dr, du))
+    assert all(torch.equal(p, q) for p, q in zip(alone, both))

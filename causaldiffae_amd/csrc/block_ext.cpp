@@ -12,6 +12,7 @@
 #include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <cmath>
 #include <string>
 #include <vector>
@@ -264,25 +265,6 @@ variable_list norm_forward(Tensor* t, const NormCfg& c) {
     return out;
 }
 
-// The gradients of the vectors first .. last (of one type) as parts of one allocation: on autograd's thread an allocation costs 2 us, and up to seven of
-// them were a fifth of a small step's backward.
-void together(const variable_list& t, const bool* want, int first, int last, variable_list& g) {
-    int64_t total = 0;
-    int like = -1;
-    for (int i = first; i <= last; ++i) if (want[i]) { total += (t[i].numel() + 63) / 64 * 64; like = i; }
-    if (like < 0) return;
-    const Tensor all = fresh({total}, t[like]);
-    int64_t at = 0;
-    for (int i = first; i <= last; ++i) {
-        if (!want[i]) continue;
-        Tensor part = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), all.dtype());
-        part.unsafeGetTensorImpl()->set_storage_offset(at);
-        part.unsafeGetTensorImpl()->set_sizes_contiguous(t[i].sizes());
-        at += (t[i].numel() + 63) / 64 * 64;
-        g[i] = part;
-    }
-}
-
 struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     using Opt = std::optional<Tensor>;
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const Opt& f, const Opt& gate, const Opt& scale, const Opt& shift, const Opt& w1, const Opt& b1,
@@ -310,15 +292,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         c10::DeviceGuard on(t[T_X].device());
         bool want[T_COUNT];
         for (size_t i = 0, edge = 0; i < T_COUNT; ++i) want[i] = t[i].defined() && ctx->needs_input_grad(edge++);
-        for (int i : {T_X, T_F}) if (want[i]) g[i] = fresh(t[i].sizes(), t[i]);
-        int vec = -1, weight = -1;
-        for (int i = T_GATE; i < T_COUNT; ++i) if (want[i]) (i < T_W1 ? vec : weight) = i;
-        if (vec >= 0 && weight >= 0 && t[vec].scalar_type() == t[weight].scalar_type()) {
-            together(t, want, T_GATE, T_B2, g);
-        } else {
-            together(t, want, T_GATE, T_SHIFT, g);
-            together(t, want, T_W1, T_B2, g);
-        }
+        for (int i = 0; i < T_COUNT; ++i) if (want[i]) g[i] = fresh(t[i].sizes(), t[i]);     // (each with memory of its own: one that is kept keeps no other)
         if (none) for (int i = T_GATE; i < T_COUNT; ++i) if (g[i].defined()) g[i].zero_();
         if (none) return once(std::move(g));
         const Rows x = rows_of(t[T_X], c.C), f = rows_of(t[T_F], c.C), dr = rows_of(dr_, c.C), du = rows_of(du_, c.C);
@@ -328,7 +302,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         p.du = ptr(du.t); p.ld_du = du.pitch;
         p.dx = mptr(g[T_X]); p.df = mptr(g[T_F]); p.dgate = mptr(g[T_GATE]); p.dscale = mptr(g[T_SCALE]); p.dshift = mptr(g[T_SHIFT]);
         p.dw1 = mptr(g[T_W1]); p.db1 = mptr(g[T_B1]); p.dw2 = mptr(g[T_W2]); p.db2 = mptr(g[T_B2]);
-        p.ws_bytes = vec < 0 && weight < 0 ? 256 : cdae_resnorm_workspace_bytes(p.B, p.T, p.C);
+        p.ws_bytes = std::any_of(want + T_GATE, want + T_COUNT, [](bool w) { return w; }) ? cdae_resnorm_workspace_bytes(p.B, p.T, p.C) : 256;
         const Tensor ws = scratch(p.ws_bytes, x.t);
         p.ws = (float*)mptr(ws);
         check(cdae_resnorm_bwd(&p, stream_of(x.t)));

@@ -1026,3 +1026,12 @@ def test_residual_norm_without_vector_gradients():
         t.requires_grad_()
     both = torch.autograd.grad(call(), (x, f, *v.values()), (dr, du))
     assert all(torch.equal(p, q) for p, q in zip(alone, both))
+
+
+def test_residual_norm_gradients_own_their_memory():
+    """a gradient that is kept or saved keeps nothing else"""
+    v = vectors(3, 40, BF16, "sample", "sample", True, True)
+    got = check_norm(rnd(1, 3, 7, 40, dtype=BF16), rnd(2, 3, 7, 40, dtype=BF16), v, 1.0, True, True, "layer", dr=rnd(3, 3, 7, 40, dtype=BF16), du=rnd(4, 3, 7, 40, dtype=BF16))
+    for k, g in got.items():
+        if k.startswith("d"):
+            assert g.untyped_storage().nbytes() == g.numel() * g.element_size(), k

@@ -1035,3 +1035,26 @@ def test_residual_norm_gradients_own_their_memory():
     for k, g in got.items():
         if k.startswith("d"):
             assert g.untyped_storage().nbytes() == g.numel() * g.element_size(), k
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("act,low", [("gelu", -12.5), ("gelu_tanh", -9.0), ("silu", -80.0)])
+def test_linear_act_tails(act, low, dtype):
+    """the activation's and the slope's own accuracy where they fall towards zero: one-value rows, so z is the input, exact in fp16 too.  Relative bounds:
+    an exponential 2^t is off by (t + 2) u relative per rounding of t, of which there are at most four, everything else by a few u"""
+    z = torch.linspace(low, 9.0, 1 << 14, device=DEV).to(BF16).to(dtype).unique()[:, None]
+    x, w = z.clone().requires_grad_(), torch.ones(1, 1, dtype=dtype, device=DEV)
+    y = blk().linear_act(x, w, act=act)
+    dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+    z = z.double()
+    if act == "gelu":
+        s, t = 0.5 * torch.special.erfc(-z / math.sqrt(2)), 0.7213475204444817 * z * z
+        slope, size = s + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi), s + z.abs() * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    else:
+        a, da = (z, torch.ones_like(z)) if act == "silu" else (1.5957691216057308 * (z + 0.044715 * z ** 3), 1.5957691216057308 * (1 + 0.134145 * z * z))
+        s, t = torch.sigmoid(a), 1.4426950408889634 * a.abs()
+        slope, size = s * (1 + z * torch.sigmoid(-a) * da), s * (1 + z.abs() * torch.sigmoid(-a) * da)
+    rel = (4 * t + 32) * u
+    within("y", y.detach(), z * s, rel * (z * s).abs())
+    # (as an operand dz is rounded, and the product by one rounds no further)
+    within("dx", dx, slope, rel * size)

@@ -67,12 +67,7 @@ __device__ __forceinline__ void stv_n(T* __restrict__ p, int n, const float (&o)
 #pragma unroll
     for (int i = 0; i < V; ++i) if (i < n) st1(p[i], o[i]);
 }
-// a vector kept either in the rows' type T or in fp32 (a uniform choice)
-template <class T, int V>
-__device__ __forceinline__ void ldv_n2(const void* __restrict__ p, long off, int is32, int n, float (&o)[V]) {
-    if (is32) ldv_n<float, V>(reinterpret_cast<const float*>(p) + off, n, o);
-    else ldv_n<T, V>(reinterpret_cast<const T*>(p) + off, n, o);
-}
+// a value of a vector kept either in the rows' type T or in fp32 (a uniform choice)
 template <class T>
 __device__ __forceinline__ void st2(void* p, long off, int is32, float v) {
     if (is32) reinterpret_cast<float*>(p)[off] = v;

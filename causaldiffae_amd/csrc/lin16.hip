@@ -293,11 +293,6 @@ __device__ __forceinline__ void lin_tile(const LinArgs& p, const int block, unsi
     using No = std::false_type;
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) if (s < stages) fetch(s);
-    // Eight rounds and more of long tiles: the first round starts in eight steps of 2000 cycles, so that some CUs write their results while others multiply
-    // (16384 x 2048 -> 8192, forward after forward: 472 us in step, 441 so; with GELU and z 486 and 462; between a training pass's other launches no
-    // difference; four rounds or half the k gain nothing).
-    if (BM == 256 && block < 256 && tiles >= 2048 && stages >= 32)
-        for (int i = block >> 3 & 7; i > 0; --i) __builtin_amdgcn_s_sleep(30);
     if (stages >= SLOTS) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((SLOTS - 1) * DMAS) : "memory");
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();

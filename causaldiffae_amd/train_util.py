@@ -16,7 +16,7 @@ import numpy as np
 import torch as th
 import torch.distributed as dist
 
-from . import dist_util, logger, ops, ops_block
+from . import dist_util, logger, ops
 from ._lib import check, lib, ptr, stream
 from .resample import LossAwareSampler, UniformSampler
 
@@ -237,6 +237,7 @@ class FusedAdamWEMA:
         pass that reads it for the norm, whose factor the optimizer kernel then takes from device memory — the gradient is not written."""
         import ctypes
         if max_norm is not None:
+            from . import ops_block      # (only here: its extension belongs to one torch, and a step without clipping does without)
             ops.side_join()              # (the norm reads what ops' weight-gradient stream writes)
             norm = ops_block.grad_factor([self.flat.grad], max_norm, grad_scale)
         self.t += 1
@@ -304,6 +305,8 @@ class TrainLoop:
         if not grad_clip >= 0.0:
             raise ValueError(f"grad_clip is the largest global gradient norm of a step, or 0 for none (got {grad_clip})")
         self.grad_clip = float(grad_clip)
+        if self.grad_clip:
+            from . import ops_block      # noqa: F401  (where its extension does not load: here, not after the first backward pass)
         if use_fp16:       # reduced-precision torso; fp32 master weights are the only weights, bf16 gradients need no loss scaling
             model.convert_to_fp16()        # marks THIS model (the mode is scoped to its forward / backward, not process-wide)
         self.model, self.diffusion, self.data = model, diffusion, data

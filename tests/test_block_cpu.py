@@ -1,6 +1,9 @@
 """Refusals and sizes of the feed-forward block's entry points that are decided on the host, before any launch (no GPU)."""
 import array
 import ctypes
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -125,3 +128,20 @@ def test_host_tensors_are_refused():
 def test_norm_scratch_stays_beside_the_rows(B, T, C):
     """with a vector for every row the column sums of all samples would be many times the rows: the backward keeps 64 MB, or less than one tensor of 16-bit rows"""
     assert 16 * C <= lib.cdae_resnorm_workspace_bytes(B, T, C) <= (64 << 20) + 2 * B * T * C
+
+
+def test_training_without_clipping_needs_no_extension():
+    """where the extension does not load, the trainer does, and only a bound on the gradients asks for it"""
+    code = """
+import sys
+sys.modules["causaldiffae_amd._block_ext"] = None
+from causaldiffae_amd import train_util
+import improved_diffusion.train_util
+kw = dict(model=None, diffusion=None, data=None, batch_size=1, microbatch=1, lr=0.0, ema_rate="0", log_interval=1, save_interval=1, resume_checkpoint="")
+try:
+    train_util.TrainLoop(**kw, grad_clip=1.0)
+except ImportError as e:
+    print("refused:", e)
+"""
+    done = subprocess.run([sys.executable, "-c", code], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "refused: causaldiffae_amd/_block_ext.so does not load" in done.stdout, (done.stdout, done.stderr[-2000:])

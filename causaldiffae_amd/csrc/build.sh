@@ -31,14 +31,17 @@ for f in build/*; do
 done
 $HIPCC --offload-arch=gfx950 -shared -fPIC -o $OUT $objs
 echo "built $(realpath $OUT)"
-# the tensor side of ops_block (host code only): calls libcdae.so, which lies beside it
+# the tensor side of ops_block (host code only): calls libcdae.so, which lies beside it.  Bound to the torch it is compiled against: built again for another
 EXT=../_block_ext.so
-if [ "${FORCE:-0}" = 1 ] || [ ! -f $EXT ] || [ block_ext.cpp -nt $EXT ] || [ ../../include/cdae.h -nt $EXT ]; then
-    TORCH=$(python3 -c 'import importlib.util, os; print(os.path.dirname(importlib.util.find_spec("torch").origin))')
-    PYINC=$(python3 -c 'import sysconfig; print(sysconfig.get_paths()["include"])')
+TORCH=$(python3 -c 'import importlib.util, os; print(os.path.dirname(importlib.util.find_spec("torch").origin))')
+PYINC=$(python3 -c 'import sysconfig; print(sysconfig.get_paths()["include"])')
+WITH="torch $(sed -n "s/^__version__ = '\(.*\)'/\1/p" "$TORCH/version.py") $PYINC"
+if [ "${FORCE:-0}" = 1 ] || [ ! -f $EXT ] || [ block_ext.cpp -nt $EXT ] || [ ../../include/cdae.h -nt $EXT ] || [ "$(cat build/.ext 2>/dev/null || true)" != "$WITH" ]; then
+    rm -f build/.ext
     g++ -O2 -std=c++17 -fPIC -shared -fvisibility=hidden -D__HIP_PLATFORM_AMD__=1 -DUSE_ROCM=1 -I"$PYINC" -isystem "$TORCH/include" \
         -isystem "$TORCH/include/torch/csrc/api/include" -isystem /opt/rocm/include -I../../include block_ext.cpp -o $EXT.new -L.. -lcdae \
         -Wl,-rpath,'$ORIGIN' -L"$TORCH/lib" -lc10 -lc10_hip -ltorch_cpu -ltorch -ltorch_python
     mv $EXT.new $EXT
+    echo "$WITH" > build/.ext
 fi
 echo "built $(realpath $EXT)"

@@ -145,3 +145,9 @@ except ImportError as e:
 """
     done = subprocess.run([sys.executable, "-c", code], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), capture_output=True, text=True, timeout=300)
     assert done.returncode == 0 and "refused: causaldiffae_amd/_block_ext.so does not load" in done.stdout, (done.stdout, done.stderr[-2000:])
+
+
+def test_extension_is_built_for_this_torch():
+    """the build records which torch the extension was compiled against, and builds it again for another"""
+    with open(os.path.join(os.path.dirname(ops_block.__file__), "csrc", "build", ".ext")) as f:
+        assert f.read().split()[:2] == ["torch", torch.__version__]

@@ -190,9 +190,10 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
             return once(std::move(g));
         }
         const Rows x = rows_of(xt, K), w = rows_of(wt, K), dy = rows_of(dy_, N);
+        const Tensor zd = z.defined() ? z.contiguous() : z;                  // (a hook on saved tensors may hand them back in another layout)
         const size_t need = linear_scratch(CDAE_LIN16_BWD, x, w, M);
         const Tensor ws = scratch(need, xt);
-        check(cdae_lin16_bwd(ptr(dy.t), dy.pitch, ptr(x.t), x.pitch, ptr(w.t), w.pitch, ptr(z), N, mptr(g[0]), K, mptr(g[1]), K, mptr(g[2]), (int)M, (int)N, (int)K,
+        check(cdae_lin16_bwd(ptr(dy.t), dy.pitch, ptr(x.t), x.pitch, ptr(w.t), w.pitch, ptr(zd), N, mptr(g[0]), K, mptr(g[1]), K, mptr(g[2]), (int)M, (int)N, (int)K,
                              (int)ctx->saved_data["act"].toInt(), type_of(xt), mptr(ws), need, stream_of(xt)));
         return once(std::move(g));
     }
@@ -279,7 +280,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         variable_list g(T_COUNT + 1);
-        const variable_list t = ctx->get_saved_variables();
+        variable_list t = ctx->get_saved_variables();
         const std::vector<int64_t> n = ctx->saved_data["n"].toIntVector();
         const std::vector<double> s = ctx->saved_data["s"].toDoubleVector();
         const NormCfg c{n[0], n[1], n[2], s[0], s[1], n[3] != 0, n[4] != 0, n[5] != 0};
@@ -297,6 +298,8 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         if (none) return once(std::move(g));
         const Rows x = rows_of(t[T_X], c.C), f = rows_of(t[T_F], c.C), dr = rows_of(dr_, c.C), du = rows_of(du_, c.C);
         const long pitch[2] = {x.pitch, f.pitch};
+        t[T_X] = x.t; t[T_F] = f.t;                                           // (a hook on saved tensors may hand them back in another layout)
+        for (int i = T_GATE; i < T_COUNT; ++i) t[i] = side_by_side(t[i]);
         cdae_resnorm p = norm_args(t.data(), pitch, c);
         p.dr = ptr(dr.t); p.ld_dr = dr.pitch;
         p.du = ptr(du.t); p.ld_du = du.pitch;

@@ -1058,3 +1058,21 @@ def test_linear_act_tails(act, low, dtype):
     within("y", y.detach(), z * s, rel * (z * s).abs())
     # (as an operand dz is rounded, and the product by one rounds no further)
     within("dx", dx, slope, rel * size)
+
+
+def test_saved_tensors_that_come_back_in_another_layout():
+    """hooks on saved tensors (offloading, compression) may hand back the same values in any layout"""
+    def other_layout(t):
+        return t.mT.contiguous().mT if t.dim() > 1 else torch.stack([t, t], -1)[:, 0]
+
+    x, w, b = rnd(1, 3, 10, 40, dtype=BF16), rnd(2, 24, 40, dtype=BF16, scale=0.2), rnd(3, 24, dtype=BF16)
+    f, dr, du, v = rnd(4, 3, 10, 40, dtype=BF16), rnd(5, 3, 10, 40, dtype=BF16), rnd(6, 3, 10, 40, dtype=BF16), vectors(3, 40, BF16, "sample", "sample", True, True)
+    leaves = [t.requires_grad_() for t in (x, f, *v.values())]
+    linear = lambda: torch.autograd.grad(blk().linear_act(x, w, b, act="gelu"), (x, w, b), rnd(7, 3, 10, 24, dtype=BF16))
+    norm = lambda: torch.autograd.grad(blk().residual_norm(x, f, gate=v["gate"], post=(v["w1"], v["b1"]), pre=(v["w2"], v["b2"]), scale=v["scale"], shift=v["shift"]), leaves, (dr, du))
+    w.requires_grad_(), b.requires_grad_()
+    for run in (linear, norm):
+        want = run()
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, other_layout):
+            got = run()
+        assert all(torch.equal(p, q) for p, q in zip(got, want)), run

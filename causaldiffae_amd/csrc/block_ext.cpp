@@ -390,7 +390,7 @@ struct List {
     }
     void read_dense() {
         for (Tensor& x : t) {
-            x = as_written(x.is_neg() ? x.detach() : x);
+            if (x.is_neg()) x = x.detach().resolve_neg();
             if (!dense(x)) x = x.detach().contiguous();
         }
     }
@@ -441,7 +441,7 @@ Tensor clip_grad_norm(const py::object& grads, double max_norm, double scale, co
         } else {
             REFUSE(a.sizes() == b.sizes() && b.device() == src.dev, who, ": outputs of the gradients' shapes, on their device");
             REFUSE(dense(b) && !b.is_neg(), who, ": outputs without gaps, their values as they are");
-            a = as_written(a);
+            if (a.is_neg()) a = a.resolve_neg();
             if (!(a.is_contiguous() && b.is_contiguous()) && !(dense(a) && a.strides() == b.strides())) a = at::empty_strided(b.sizes(), b.strides(), a.options()).copy_(a);
         }
     }

@@ -447,6 +447,9 @@ __global__ __launch_bounds__(256) void lin_pad_kernel(const PadJobs jobs) {
 // columns x 8 lanes of rows, 8 columns a thread, one row at a time (8192 x 1536 with GELU, sums only: 14.2 us; two rows in flight 15.9, four 17.7, eight
 // 29.3: the waves' number is worth more than their registers).  Loads and stores have no branches around them: the last thread of a row takes the row's
 // LAST 8 values (its neighbour's are among them, written twice with the same value and summed once).  SMALL: rows of fewer than 8 values.
+// dz is written in the rows' type because the matrix instructions take both operands in one 16-bit type.  That rounding is a second one, independent of the
+// result's: relative to 64 bits dx and dw are 2.35e-3 off in bf16 and 3.0e-4 in fp16, where one rounding leaves 1.66e-3 and 2.1e-4 (measured at 8192 x 384 ->
+// 1536 and 1021 x 393 -> 771).  A second operand with what the rounding drops would remove it and double both products.  The sums take dz unrounded.
 template <class T, bool SMALL>
 __global__ __launch_bounds__(256) void lin_slope_kernel(const T* __restrict__ dy, long lddy, const F16* __restrict__ z, long ldz, T* __restrict__ dz, long lddz,
                                                         float* __restrict__ part, T* __restrict__ db, int M, int N, int rows_per_block, int ncb, int act) {
@@ -512,13 +515,14 @@ bool al16(const void* p) { return ((size_t)p & 15) == 0; }
 size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 
 // Tile, slots and splits of the sum over k: the cheapest by what a stage of 64 k and a tile's beginning and end cost (us), as measured on bf16 operands:
-//     256 x 256, one block a CU                    1.5   9      16384 x 2048 x 8192 weight gradient, 256 tiles of 256 stages: 384 us (128 x 128 532)
-//     128 x 128, four slots, one block a CU        0.5   3      8192 x 2048 -> 512 forward, 256 tiles of 32 stages: 19.3 us (two slots 24.3, 64 x 64 26.5)
-//     128 x 128, two slots, two blocks a CU        1.03  2.7    8192 x 384 -> 1536 forward, 768 tiles of 6 stages: 17.8 us (256 x 256 18.7, 64 x 64 24.1)
-//     64 x 64, one block a CU                      0.26  2.5    1024 x 392 -> 768 data gradient, 112 tiles of 12 stages: 6.3 us (128 x 128 10.7)
-//     64 x 64, two blocks a CU                     0.38  3.5    2048 x 1024 -> 1024 forward, 512 tiles of 16 stages: 8.4 us (128 x 128 11.4)
-// A split costs a second launch (3.5) and its partial sums twice (6 TB/s): 1536 x 384 over 8192 rows 26.8 us in seven splits, 64.1 in one, 36.5 in
-// fourteen; 2048 x 1024 over 1024 rows 11.2 in one, 16.8 in two.
+//     256 x 256, one block a CU                    1.5   9      16384 x 2048 x 8192 weight gradient, 256 tiles of 256 stages: 390 us (128 x 128 521)
+//     128 x 128, four slots, one block a CU        0.5   3      8192 x 2048 -> 512 forward, 256 tiles of 32 stages: 21.3 us (two slots 25.1, 64 x 64 28.3, 256 x 256 42.4)
+//     128 x 128, two slots, two blocks a CU        1.03  2.7    8192 x 384 -> 1536 forward, 768 tiles of 6 stages: 18.6 us (256 x 256 18.6, 64 x 64 25.8)
+//     64 x 64, one block a CU                      0.26  2.5    1024 x 392 -> 768 data gradient, 112 tiles of 12 stages: 6.6 us (128 x 128 10.8)
+//     64 x 64, two blocks a CU                     0.38  3.5    2048 x 1024 -> 1024 forward, 512 tiles of 16 stages: 9.4 us (128 x 128 12.1)
+// (kernel times, launch after launch on the same operands; with other work between them the forward of 8192 x 2048 -> 512 with a residual takes 25.2.)
+// A split costs a second launch (3.5) and its partial sums twice (6 TB/s): 1536 x 384 over 8192 rows 27.0 us in seven splits, 33.6 in one; 2048 x 1024 over
+// 1024 rows 10.2 in one, 22.8 in two.
 // (A call works its plan out anew, twice with the question for the workspace, so this is host time of every call: tables first, then the combinations.)
 struct Kind { int bm, slots, at_once; double stage, ends; };
 const Kind kinds[] = {{256, 2, 256, 1.5, 9.0}, {128, 4, 256, 0.5, 3.0}, {128, 2, 512, 1.03, 2.7}, {64, 4, 256, 0.26, 2.5}, {64, 4, 512, 0.38, 3.5}};
@@ -554,7 +558,7 @@ Plan plan(int M, int N, int K) {
 }
 // A backward's two products: dx [M][K] over N, dw [N][K] over M, each by its own plan, or together on one kind of tile where that is cheaper by the same
 // model (a launch that keeps all slots busy takes its blocks' time over the slots, and half a block for its end).
-// 8192 x 384 -> 1536: 36 us together, 49 one after the other (traced).
+// 8192 x 384 -> 1536: 34 us together, 44 one after the other (traced).
 struct Pair { Plan x, w; bool together; int bm, slots, sx, sw; };
 Pair pair_plan(int M, int N, int K) {
     constexpr int S = 8;

@@ -8,12 +8,14 @@
 A block is residual_norm -> linear_act (activation) -> linear_act -> residual_norm: the second residual_norm closes this block and opens the next.
 Rows are the last dimension: an activation [N, C, H, W] in this package's NHWC storage is passed as x.permute(0, 2, 3, 1).
 
-Sums, statistics and products accumulate in fp32 (the norm of the gradients in fp64) and every result is rounded once.  Calls run on the current
-stream of their tensors' device, allocate their scratch themselves for the one call, neither synchronise nor copy to the host, keep nothing between
-calls and can be captured into a graph.  (A backward pass can be captured only while no eager graph over the same leaves, made on the default stream,
-is alive: the captured forward raises then.)  Gradients are first derivatives; a second one raises, and so does an input that
-carries a forward-mode tangent.  Wrong tensors and values raise CdaeError; there is
-no CPU form.  The checks and the autograd nodes are native (csrc/block_ext.cpp): the kernels of a call are shorter than the same dispatch from Python.
+Sums, statistics and products accumulate in fp32 (the norm of the gradients in fp64) and every result is rounded once.  linear_act's backward rounds twice
+more in between, both named there: with an activation, its gradients of x and w are 1.4 times as far from the exact ones as one rounding would leave them.
+
+Calls run on the current stream of their tensors' device, allocate their scratch themselves for the one call, neither synchronise nor copy to the host,
+keep nothing between calls and can be captured into a graph.  (A backward pass is captured together with its forward, and only while no eager graph over the
+same leaves, made on the default stream, is alive: the captured forward raises then.)  Gradients are first derivatives; a second one raises, and so does an
+input that carries a forward-mode tangent.  Wrong tensors and values raise CdaeError; there is no CPU form.  The checks and the autograd nodes are native
+(csrc/block_ext.cpp): the kernels of a call are shorter than the same dispatch from Python.
 """
 import torch
 
@@ -31,8 +33,9 @@ MAX_FEATURES = 8192          # widest row of residual_norm
 
 def linear_act(x, w, b=None, res=None, act="none"):
     """y = act(x @ w^T + b) + res for rows x [..., K], a weight [N, K], a bias [N] and a residual [..., N], all bf16 or all fp16; y has their type.
-    act: "none", "silu", "relu", "gelu" or "gelu_tanh".  Where a gradient is wanted the pre-activation is kept in fp16 beside x and w.  Rows at any
-    pitch and alignment are taken; fp32 rows belong to ops.linear."""
+    act: "none", "silu", "relu", "gelu" or "gelu_tanh".  With an activation, where a gradient is wanted, the pre-activation is kept in fp16 beside x and w, and
+    the gradient dz that it leads to is rounded to the rows' type as an operand of the products that give dx and dw (the bias gradient adds it unrounded).
+    Rows at any pitch and alignment are taken; fp32 rows belong to ops.linear."""
     return _ext.linear_act(x, w, b, res, act)
 
 
